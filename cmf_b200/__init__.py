@@ -8,7 +8,7 @@ the engine's function names and argument meaning.  There is no CPU fallback: eve
 either runs on the device or raises :class:`CmfCudaError`.
 """
 from ._lib import CmfCudaError, lib, library_path  # noqa: F401
-from . import gpu  # noqa: F401
+from . import gpu, ops  # noqa: F401
 from .container import CmfWriter, Model  # noqa: F401
 from .dit import NextDit, GenParams, denoise  # noqa: F401
 from .vae import VaeDecoder  # noqa: F401

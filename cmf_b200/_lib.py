@@ -90,6 +90,13 @@ SYMBOLS = {
     "cmfc_encode_random": (C.c_int, [C.c_int, C.c_uint64, C.c_float, C.c_size_t, C.c_size_t, C.c_void_p]),
     "cmfc_noalloc_max_elements": (C.c_size_t, []),
     "cmfc_matmat_device_noalloc": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "cmfc_quantize_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_int64, C.c_void_p, C.c_int64,
+                                     C.c_void_p, C.c_void_p]),
+    "cmfc_i8_matmat": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t,
+                                 C.c_size_t, C.c_size_t, C.c_void_p, C.c_int, C.c_int64, C.c_void_p]),
+    "cmfc_q8_matmat_i8": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p]),
+    "cmfc_qk_norm_rope": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p]),
+    "cmfc_window_attention": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p]),
     "cmfc_selftest_wait_timeout": (C.c_int, [C.c_uint32]),
     "cmfc_launch_count": (C.c_uint64, [C.c_int]),
     "cmfc_bench_gemm": (C.c_int, [C.c_void_p, C.c_int64, C.c_size_t, C.c_int, C.c_int, C.POINTER(C.c_float)]),

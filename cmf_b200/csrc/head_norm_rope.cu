@@ -1,0 +1,288 @@
+// Norms of query and key heads with the position rotation in the same pass, and the row quantizer of
+// the 8-bit products: bandwidth-bound row kernels on the caller's device tensors.
+//
+// Per (token, head): y = x / sqrt(mean(x^2) + eps) * w, then every pair (a, b) of the first `rot`
+// dims becomes (a c - b s, a s + b c) with c, s of the token's position; the other dims pass through.
+// Pairs are neighbours (2i, 2i + 1) or halves (i, i + rot / 2).  Statistics and arithmetic are f32,
+// the result is rounded once to the tensors' type.
+//
+// Bound: memory.  A head is read once and written once; the norm's gain and the position's cos / sin
+// are read once per (token, up to HEADS_PER_ITEM heads) and stay in registers.  A lane owns two
+// 16-byte chunks of a head that hold both members of its pairs (neighbouring chunks, or the same
+// chunk of either half), so the rotation needs no exchange between lanes; a head takes a group of
+// 4 to 32 lanes and a warp works on 32 / group items.
+#include "text_ops.cuh"
+
+namespace cmfc {
+namespace {
+
+constexpr int HEADS_PER_ITEM = 4;
+
+// N (a multiple of 4) values from a 16-byte aligned place
+template <int N>
+__device__ __forceinline__ void load_f32(const float* p, float* o) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p + i));
+        o[i] = v.x;
+        o[i + 1] = v.y;
+        o[i + 2] = v.z;
+        o[i + 3] = v.w;
+    }
+}
+
+template <typename T, bool HALF, int LANES>
+__global__ void __launch_bounds__(128) norm_rope_kernel(NormRopeParams p, int heads_per_item, int q_items, int items_per_token) {
+    constexpr int V = 16 / sizeof(T);  // elements of a 16-byte chunk
+    const int u = threadIdx.x % LANES;                 // this lane's unit: two chunks, V pairs
+    const int units = p.hd / (2 * V), rot_units = p.rot / (2 * V);
+    const int64_t item = (int64_t)blockIdx.x * (128 / LANES) + threadIdx.x / LANES;
+    const bool active = u < units && item < p.n * items_per_token;
+    const int64_t t = active ? item / items_per_token : 0;
+    const int part = active ? (int)(item % items_per_token) : 0;
+    const bool is_q = part < q_items;
+    const int head0 = (is_q ? part : part - q_items) * heads_per_item;
+    const int heads = active ? min(heads_per_item, (is_q ? p.nh : p.nkv) - head0) : 0;
+    const HeadView in = is_q ? p.q : p.k, out = is_q ? p.q_out : p.k_out;
+    const bool rotated = u < rot_units;
+    const int d0 = HALF && rotated ? u * V : u * 2 * V;
+    const int d1 = HALF && rotated ? p.rot / 2 + u * V : d0 + V;
+    float w[2 * V], cs[V], sn[V];
+    bool bad = false;
+    if (active) {
+        const float* g = is_q ? p.norm_q : p.norm_k;
+        load_f32<V>(g + d0, w);
+        load_f32<V>(g + d1, w + V);
+        const int64_t pos = p.positions ? (p.pos64 ? static_cast<const int64_t*>(p.positions)[t]
+                                                   : (int64_t)static_cast<const int32_t*>(p.positions)[t])
+                                        : t;
+        bad = pos < 0 || pos >= p.table_rows;
+        if (rotated && !bad) {
+            load_f32<V>(p.cos_t + pos * (p.rot / 2) + u * V, cs);
+            load_f32<V>(p.sin_t + pos * (p.rot / 2) + u * V, sn);
+        }
+    }
+    const T* src = static_cast<const T*>(in.p) + t * in.row + (int64_t)head0 * in.head;
+    T* dst = static_cast<T*>(const_cast<void*>(out.p)) + t * out.row + (int64_t)head0 * out.head;
+    uint4 raw[HEADS_PER_ITEM][2];
+#pragma unroll
+    for (int h = 0; h < HEADS_PER_ITEM; ++h)
+        if (h < heads) {
+            raw[h][0] = *reinterpret_cast<const uint4*>(src + h * in.head + d0);
+            raw[h][1] = *reinterpret_cast<const uint4*>(src + h * in.head + d1);
+        }
+#pragma unroll
+    for (int h = 0; h < HEADS_PER_ITEM; ++h) {
+        // every lane of the warp takes part in the group's sum, with nothing to add where it has no head
+        if (h >= heads_per_item) break;
+        float x[2 * V], ss = 0.0f;
+        if (h < heads) {
+            unpack16<T>(raw[h][0], x);
+            unpack16<T>(raw[h][1], x + V);
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) ss = fmaf(x[i], x[i], ss);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (h >= heads) continue;
+        const float inv = bad ? __int_as_float(0x7fc00000) : 1.0f / sqrtf(ss / (float)p.hd + p.eps);
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) x[i] = (x[i] * inv) * w[i];
+        if (rotated && !bad) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float& a = HALF ? x[i] : x[2 * i];
+                float& b = HALF ? x[V + i] : x[2 * i + 1];
+                const float ra = fmaf(a, cs[i], -(b * sn[i])), rb = fmaf(a, sn[i], b * cs[i]);
+                a = ra;
+                b = rb;
+            }
+        }
+        *reinterpret_cast<uint4*>(dst + h * out.head + d0) = pack16<T>(x);
+        *reinterpret_cast<uint4*>(dst + h * out.head + d1) = pack16<T>(x + V);
+    }
+}
+
+// Any head size, rotation, stride and alignment: one warp per (token, head), a pair per lane.
+// Lane i reads and writes the same pairs, so an output that is the input itself is fine here too.
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(128) norm_rope_any_kernel(NormRopeParams p) {
+    const int lane = threadIdx.x & 31;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int all = p.nh + p.nkv;
+    if (item >= p.n * all) return;
+    const int64_t t = item / all;
+    const int hh = (int)(item % all);
+    const bool is_q = hh < p.nh;
+    const int h = is_q ? hh : hh - p.nh;
+    const HeadView in = is_q ? p.q : p.k, out = is_q ? p.q_out : p.k_out;
+    const float* g = is_q ? p.norm_q : p.norm_k;
+    const T* src = static_cast<const T*>(in.p) + t * in.row + (int64_t)h * in.head;
+    T* dst = static_cast<T*>(const_cast<void*>(out.p)) + t * out.row + (int64_t)h * out.head;
+    float ss = 0.0f;
+    for (int d = lane; d < p.hd; d += 32) {
+        const float x = to_f32(src[d]);
+        ss = fmaf(x, x, ss);
+    }
+    ss = warp_sum(ss);
+    const int64_t pos = p.positions ? (p.pos64 ? static_cast<const int64_t*>(p.positions)[t]
+                                               : (int64_t)static_cast<const int32_t*>(p.positions)[t])
+                                    : t;
+    const bool bad = pos < 0 || pos >= p.table_rows;
+    const float inv = bad ? __int_as_float(0x7fc00000) : 1.0f / sqrtf(ss / (float)p.hd + p.eps);
+    __syncwarp();  // the sums have read what the loops below overwrite when the output is the input
+    const int half = p.rot / 2;
+    for (int i = lane; i < half; i += 32) {
+        const int da = HALF ? i : 2 * i, db = HALF ? i + half : 2 * i + 1;
+        const float a = (to_f32(src[da]) * inv) * g[da], b = (to_f32(src[db]) * inv) * g[db];
+        const float c = bad ? 1.0f : p.cos_t[pos * half + i], s = bad ? 0.0f : p.sin_t[pos * half + i];
+        dst[da] = from_f32<T>(fmaf(a, c, -(b * s)));
+        dst[db] = from_f32<T>(fmaf(a, s, b * c));
+    }
+    for (int d = p.rot + lane; d < p.hd; d += 32) dst[d] = from_f32<T>((to_f32(src[d]) * inv) * g[d]);
+}
+
+template <typename T, bool HALF, int LANES>
+void norm_rope_lanes(const NormRopeParams& p, cudaStream_t s) {
+    // few tokens: a head per lane group, so that the heads spread over the SMs (one token of 24 + 8
+    // heads); many: four heads share the gain and the rotation that a group holds in registers
+    const int per = p.n * (p.nh + p.nkv) >= 16384 ? HEADS_PER_ITEM : 1;
+    const int q_items = (p.nh + per - 1) / per, items = q_items + (p.nkv + per - 1) / per;
+    const int64_t groups = p.n * items, per_block = 128 / LANES;
+    norm_rope_kernel<T, HALF, LANES><<<(unsigned)((groups + per_block - 1) / per_block), 128, 0, s>>>(p, per, q_items, items);
+}
+
+template <typename T, bool HALF>
+void norm_rope_typed(const NormRopeParams& p, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    auto fits = [](const HeadView& v) {
+        return (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.row % V == 0 && v.head % V == 0;
+    };
+    auto aligned = [](const float* f) { return (reinterpret_cast<uintptr_t>(f) & 15) == 0; };
+    const int units = p.hd / (2 * V);
+    // the 16-byte form needs aligned rows, heads, gains and tables, and whole units of two chunks (rot / 2
+    // is then a multiple of V, so every table row starts on 16 bytes too)
+    if (p.hd % (2 * V) || p.rot % (2 * V) || units > 32 || !aligned(p.cos_t) || !aligned(p.sin_t) ||
+        (p.nh && !aligned(p.norm_q)) || (p.nkv && !aligned(p.norm_k)) || (p.nh && !(fits(p.q) && fits(p.q_out))) ||
+        (p.nkv && !(fits(p.k) && fits(p.k_out)))) {
+        const int64_t items = p.n * (p.nh + p.nkv);
+        norm_rope_any_kernel<T, HALF><<<(unsigned)((items + 3) / 4), 128, 0, s>>>(p);
+    } else if (units <= 4) {
+        norm_rope_lanes<T, HALF, 4>(p, s);
+    } else if (units <= 8) {
+        norm_rope_lanes<T, HALF, 8>(p, s);
+    } else if (units <= 16) {
+        norm_rope_lanes<T, HALF, 16>(p, s);
+    } else {
+        norm_rope_lanes<T, HALF, 32>(p, s);
+    }
+}
+
+// ---------------- rows to 8 bits ----------------
+// scale = max |x| / 127, q = rint(x / scale) (ties to even), both quotients IEEE f32.  A row of zeros
+// (or one whose scale underflows to zero) gives scale 0 and levels 0; a row that holds an infinity or a
+// NaN gives levels 0 and scale NaN, so that every product with it is NaN.
+// One block per row: the row is read once into registers (CACHED chunks per thread; what does not fit
+// is read again, from L2), so traffic is the input and the levels.
+constexpr int QUANT_THREADS = 256;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t cols,
+                                                                      int8_t* __restrict__ q, int64_t ldq,
+                                                                      float* __restrict__ scale) {
+    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+    constexpr int CACHED = VEC ? 4 : 8;
+    const int64_t r = blockIdx.x;
+    const T* src = x + r * ldx;
+    int8_t* dst = q + r * ldq;
+    const int64_t chunks = cols / V;
+    __shared__ unsigned red[QUANT_THREADS / 32];
+    float v[CACHED][V];
+    unsigned top = 0;  // of the bit patterns of |x|: NaN above infinity above every number
+    auto fetch = [&](int64_t c, float (&o)[V]) {
+        if constexpr (VEC) unpack16<T>(*reinterpret_cast<const uint4*>(src + c * V), o);
+        else o[0] = to_f32(src[c]);
+    };
+#pragma unroll
+    for (int i = 0; i < CACHED; ++i) {
+        const int64_t c = threadIdx.x + (int64_t)i * QUANT_THREADS;
+        if (c < chunks) {
+            fetch(c, v[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[i][e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+    }
+    for (int64_t c = threadIdx.x + (int64_t)CACHED * QUANT_THREADS; c < chunks; c += QUANT_THREADS) {
+        float o[V];
+        fetch(c, o);
+#pragma unroll
+        for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(o[e]) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < QUANT_THREADS / 32; ++i) top = max(top, red[i]);
+    const bool finite = top < 0x7f800000u;
+    const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __int_as_float(0x7fc00000);
+    const bool zero = !finite || s == 0.0f;
+    if (threadIdx.x == 0) scale[r] = s;
+    // a scale rounded down among the subnormals could let the largest quotient pass 127
+    auto level = [&](float f) { return zero ? 0 : max(-127, min(127, __float2int_rn(__fdiv_rn(f, s)))); };
+    auto put = [&](int64_t c, const float (&o)[V]) {
+        if constexpr (VEC) {
+            uint32_t w[V / 4];
+#pragma unroll
+            for (int e = 0; e < V; e += 4)
+                w[e / 4] = (uint32_t)(uint8_t)level(o[e]) | (uint32_t)(uint8_t)level(o[e + 1]) << 8 |
+                           (uint32_t)(uint8_t)level(o[e + 2]) << 16 | (uint32_t)(uint8_t)level(o[e + 3]) << 24;
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(dst + c * V) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t*>(dst + c * V) = w[0];
+        } else {
+            dst[c] = (int8_t)level(o[0]);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < CACHED; ++i) {
+        const int64_t c = threadIdx.x + (int64_t)i * QUANT_THREADS;
+        if (c < chunks) put(c, v[i]);
+    }
+    for (int64_t c = threadIdx.x + (int64_t)CACHED * QUANT_THREADS; c < chunks; c += QUANT_THREADS) {
+        float o[V];
+        fetch(c, o);
+        put(c, o);
+    }
+}
+
+template <typename T>
+void quantize_rows_typed(const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !(reinterpret_cast<uintptr_t>(q) & 7) && cols % V == 0 && ldx % V == 0 && ldq % V == 0;
+    const T* xt = static_cast<const T*>(x);
+    if (vec) quantize_rows_kernel<T, true><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, cols, q, ldq, scale);
+    else quantize_rows_kernel<T, false><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, cols, q, ldq, scale);
+}
+
+}  // namespace
+
+int launch_norm_rope(const NormRopeParams& p, int elem, bool half_split, cudaStream_t s) {
+    if (elem == ET_F32) half_split ? norm_rope_typed<float, true>(p, s) : norm_rope_typed<float, false>(p, s);
+    else if (elem == ET_F16) half_split ? norm_rope_typed<__half, true>(p, s) : norm_rope_typed<__half, false>(p, s);
+    else half_split ? norm_rope_typed<__nv_bfloat16, true>(p, s) : norm_rope_typed<__nv_bfloat16, false>(p, s);
+    CMFC_CUDA(cudaGetLastError());
+    return OK;
+}
+
+int launch_quantize_rows(const void* x, int elem, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                         cudaStream_t s) {
+    if (elem == ET_F32) quantize_rows_typed<float>(x, rows, cols, ldx, q, ldq, scale, s);
+    else if (elem == ET_F16) quantize_rows_typed<__half>(x, rows, cols, ldx, q, ldq, scale, s);
+    else quantize_rows_typed<__nv_bfloat16>(x, rows, cols, ldx, q, ldq, scale, s);
+    CMFC_CUDA(cudaGetLastError());
+    return OK;
+}
+
+}  // namespace cmfc

@@ -196,6 +196,26 @@ Context* ctx_existing() {
     return it == g_ctxs.end() ? nullptr : it->second.get();
 }
 
+Context* ctx_of_device(int device, cudaStream_t stream) {
+    {
+        std::lock_guard<std::mutex> lk(g_ctx_mu);
+        auto it = g_ctxs.find(device);
+        if (it != g_ctxs.end()) return it->second.get();
+    }
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
+        // a context allocates and synchronizes, which would invalidate the capture
+        fail(ERR_BAD_ARG, "the first call on a device must not be captured into a graph; call it (or cmfc_set_device) once before");
+        return nullptr;
+    }
+    const int lib_device = g_cur_device;
+    const int rc = ctx_set_device(device);
+    g_cur_device = lib_device;
+    if (rc != OK) return nullptr;
+    std::lock_guard<std::mutex> lk(g_ctx_mu);
+    return g_ctxs[device].get();
+}
+
 int check_status(Context* c, const char* what) {
     CMFC_CUDA(cudaMemcpyAsync(c->status_host, c->status, 4, cudaMemcpyDeviceToHost, c->stream));
     CMFC_CUDA(cudaStreamSynchronize(c->stream));

@@ -124,6 +124,9 @@ const std::string& last_error();
 Context* ctx();  // context of the calling thread's current device (created on demand), or null
 Context* ctx_existing();  // same, but never creates a context (and so never allocates)
 int ctx_set_device(int device);
+// context of `device`, which is current, created on first use without changing the library's current
+// device; null (with the thread's message set) when it cannot be made, as while `stream` is being captured
+Context* ctx_of_device(int device, cudaStream_t stream);
 int check_status(Context* c, const char* what);  // reads the device status word (after a sync)
 
 // weights

@@ -1,0 +1,140 @@
+// Shared by the windowed-attention kernels: which rows and keys a block works on, the mask and the score.
+#pragma once
+#include "text_ops.cuh"
+
+namespace cmfc {
+
+int launch_window_any(const WindowAttnParams& p, int elem, cudaStream_t s);
+
+// Upper bound of the row tiles of all sequences: every sequence adds at most one partial tile.
+inline int64_t max_tiles(const WindowAttnParams& p, int rows_per_tile) {
+    return p.q_rows * (p.nh / p.nkv) / rows_per_tile + p.seqs;
+}
+
+#ifdef __CUDACC__
+
+struct SeqTile {
+    int64_t q0, k0;     // first query row, first key row
+    int q_len, k_len;
+    int tile;           // row tile inside the sequence
+};
+
+// The caller's offsets are device data that the host never sees: they are clamped to the tensors, so a
+// wrong value can give wrong results but no access out of range.
+__device__ __forceinline__ void load_seq(const WindowAttnParams& p, int s, SeqTile& st) {
+    if (!p.q_start) {
+        st.q0 = st.k0 = 0;
+        st.q_len = (int)p.q_rows;
+        st.k_len = (int)p.k_rows;
+        return;
+    }
+    const int64_t a = min(max((int64_t)p.q_start[s], (int64_t)0), p.q_rows);
+    const int64_t b = min(max((int64_t)p.q_start[s + 1], a), p.q_rows);
+    st.q0 = a;
+    st.q_len = (int)(b - a);
+    st.k0 = min(max((int64_t)p.k_start[s], (int64_t)0), p.k_rows);
+    st.k_len = (int)min(max((int64_t)p.k_len[s], (int64_t)0), p.k_rows - st.k0);
+}
+
+// Sequence and row tile of number `index` in the row tiles of all sequences: every warp counts the tiles
+// of 32 sequences at a time.  False: there is no such tile (the grid is an upper bound).
+__device__ __forceinline__ bool find_tile(const WindowAttnParams& p, int64_t index, int rows_per_tile, int group, SeqTile& st) {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int s0 = 0; s0 < p.seqs; s0 += 32) {
+        SeqTile mine;
+        mine.q_len = 0;
+        if (s0 + lane < p.seqs) load_seq(p, s0 + lane, mine);
+        const int64_t tiles = ((int64_t)mine.q_len * group + rows_per_tile - 1) / rows_per_tile;
+        int64_t upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, index < before + upto);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            st.tile = (int)(index - (before + __shfl_sync(0xffffffffu, upto - tiles, src)));
+            load_seq(p, s0 + src, st);
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+// Key tiles that some query of [first_i, last_i] sees: those of the sinks, then those of the window.
+struct KeyTiles {
+    int sink_tiles, low_tile, count;
+    __device__ __forceinline__ int at(int it) const { return it < sink_tiles ? it : low_tile + (it - sink_tiles); }
+};
+__device__ __forceinline__ KeyTiles key_tiles(const WindowAttnParams& p, const SeqTile& st, int first_i, int last_i, int n) {
+    KeyTiles kt;
+    const int shift = st.k_len - st.q_len;
+    const int first = shift + first_i, last = shift + last_i;  // positions; below 0: sees nothing
+    if (last < 0) {
+        kt.sink_tiles = kt.low_tile = kt.count = 0;
+        return kt;
+    }
+    const int low = (int)max((int64_t)0, (int64_t)first - p.window + 1);  // first key of the earliest window
+    kt.low_tile = low / n;
+    const int sink_keys = min(p.sinks, low);
+    kt.sink_tiles = min((sink_keys + n - 1) / n, kt.low_tile);
+    kt.count = kt.sink_tiles + (last / n - kt.low_tile + 1);
+    return kt;
+}
+
+__device__ __forceinline__ bool sees(const WindowAttnParams& p, int pos, int j) {
+    return j <= pos && (pos - j < p.window || j < p.sinks);
+}
+__device__ __forceinline__ float score(float dot, float scale, float softcap) {
+    const float s = dot * scale;
+    return softcap > 0.0f ? softcap * tanhf(s / softcap) : s;
+}
+
+// One warp, one (query, head) row, key by key over exactly the keys that the row sees: rows whose tile
+// result is not finite come here, so that an infinity or a NaN among keys or values that the row does not
+// see cannot reach it, and one that it does see gives what the formula gives.
+template <typename T>
+__device__ __noinline__ void redo_row(const WindowAttnParams& p, const SeqTile& st, int kvh, int row) {
+    const int lane = threadIdx.x & 31;
+    const int group = p.nh / p.nkv;
+    const int64_t qi = st.q0 + row / group;
+    const int head = kvh * group + row % group;
+    const int pos = st.k_len - st.q_len + row / group;
+    const T* q = static_cast<const T*>(p.q.p) + qi * p.q.row + (int64_t)head * p.q.head;
+    const T* k = static_cast<const T*>(p.k.p) + st.k0 * p.k.row + (int64_t)kvh * p.k.head;
+    const T* v = static_cast<const T*>(p.v.p) + st.k0 * p.v.row + (int64_t)kvh * p.v.head;
+    T* out = static_cast<T*>(const_cast<void*>(p.out.p)) + qi * p.out.row + (int64_t)head * p.out.head;
+    float qv[8], acc[8], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        qv[c] = lane + 32 * c < p.hd ? to_f32(q[lane + 32 * c]) : 0.0f;
+        acc[c] = 0.0f;
+    }
+    const int low = (int)max((int64_t)0, (int64_t)pos - p.window + 1);
+    for (int j = p.sinks > 0 ? 0 : low; j <= pos; ++j) {
+        if (j >= p.sinks && j < low) j = low;
+        float dot = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (lane + 32 * c < p.hd) dot = fmaf(qv[c], to_f32(k[j * p.k.row + lane + 32 * c]), dot);
+        const float s = score(warp_sum(dot), p.scale, p.softcap);
+        const float mn = s != s ? s : fmaxf(m, s);  // a NaN score makes the row NaN
+        const float alpha = mn == m ? 1.0f : expf(m - mn), e = s == -INFINITY ? 0.0f : expf(s - mn);
+        m = mn;
+        l = l * alpha + e;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (lane + 32 * c < p.hd) acc[c] = acc[c] * alpha + e * to_f32(v[j * p.v.row + lane + 32 * c]);
+    }
+    const float inv = 1.0f / l;  // every score -inf: 0 / 0, NaN as the formula
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        if (lane + 32 * c < p.hd) out[lane + 32 * c] = from_f32<T>(acc[c] * inv);
+}
+
+#endif  // __CUDACC__
+
+}  // namespace cmfc

@@ -51,6 +51,13 @@ def q8_matmat(model: Model, idx: int, row_scale, pre, b: int, rows: int, cols: i
     return _matmat(lib().cmfc_q8_matmat, model, idx, pre, b, rows, cols, out)
 
 
+def q8_matmat_i8(model: Model, idx: int, xs, b: int, rows: int, cols: int, out) -> bool:
+    """:func:`q8_matmat` with the activations rounded to 8 bits too, one scale for each token
+    (``scale = max |x| / 127``): the product runs on the 8-bit tensor cores and its integer sums are
+    exact.  ``idx`` must be a q8_row tensor.  No counterpart in the reference."""
+    return _matmat(lib().cmfc_q8_matmat_i8, model, idx, xs, b, rows, cols, out)
+
+
 def q4t_matmat(model: Model, idx: int, xs, b: int, rows: int, cols: int, out) -> bool:
     """gpu.rs:2439"""
     return _matmat(lib().cmfc_q4t_matmat, model, idx, xs, b, rows, cols, out)

@@ -269,6 +269,80 @@ int cmfc_encode_random(int dtype, uint64_t seed, float std, size_t rows, size_t 
 size_t cmfc_noalloc_max_elements(void);
 int cmfc_matmat_device_noalloc(cmfc_model* m, int64_t idx, const float* d_x, size_t b, float* d_y);
 
+/* ---- operators of text-model attention layers on the caller's device tensors ----
+ * No counterpart in the engine's facade (its host computes these); they stand beside the entries of the
+ * same kind above: 8-bit products beside q8_matmat, windowed attention beside dit_attention, head norms
+ * with the rotation beside the pass that the denoiser runs inside its blocks.
+ *
+ * All pointers are memory of `device`; strides and pitches are in elements.  The work is enqueued on
+ * `stream` (a cudaStream_t, NULL: the legacy default stream) and the call returns at once: inputs and
+ * outputs belong to the call until that stream has passed it.  A call may be captured into a CUDA graph once
+ * the device has a context (any earlier call on it, or cmfc_set_device).  Nothing is kept between
+ * calls and no workspace is shared, so calls may overlap on several streams.  The thread's current device
+ * and the library's are left as they were.  A kernel that gives up a bounded wait leaves its code in the
+ * device's status word, which cmfc_synchronize (after the stream has been synchronized) reports. */
+
+/* element types of those tensors */
+#define CMFC_ET_F32 0
+#define CMFC_ET_F16 1
+#define CMFC_ET_BF16 2
+
+/* Rows to 8 bits: scale[r] = max_c |x[r, c]| / 127, q[r, c] = rint(x[r, c] / scale[r]) (ties to even; both
+ * quotients in f32).  A row of zeros gives scale 0 and levels 0; a row that holds an infinity or a NaN gives
+ * scale NaN and levels 0.  x [rows, cols] of type `elem`, pitch ldx; q pitch ldq; scale [rows]. */
+int cmfc_quantize_rows(int device, const void* x, int elem, size_t rows, size_t cols, int64_t ldx, int8_t* q, int64_t ldq,
+                       float* scale, void* stream);
+/* y[m, n] = (sum_k xq[m, k] wq[n, k]) * (x_scale[m] * w_scale[n]): xq [b, cols], wq [rows, cols] (a q8_row
+ * tensor's levels and row scales), y [b, rows] of type `elem`.  The sum is exact in 32-bit integers
+ * (cols <= 131071).  Fastest with pitches and bases that are multiples of 16 bytes. */
+int cmfc_i8_matmat(int device, const int8_t* xq, int64_t ldx, const float* x_scale, const int8_t* wq, int64_t ldw,
+                   const float* w_scale, size_t b, size_t rows, size_t cols, void* y, int elem, int64_t ldy, void* stream);
+/* cmfc_q8_matmat (gpu.rs:1155) with the activations rounded to 8 bits too (cmfc_quantize_rows): host f32
+ * in and out; tensor idx must be q8_row.  Runs on the library's stream and returns when done. */
+int cmfc_q8_matmat_i8(cmfc_model* m, int64_t idx, const float* xs, size_t b, size_t rows, size_t cols, float* out);
+
+/* Norms of query and key heads and the position rotation, in one pass.  For every token t < n and head:
+ *   y = x / sqrt(mean(x^2) + eps) * norm;  then the pairs (a, b) of the first `rot` dims, (2i, 2i + 1) or with
+ *   half_split (i, i + rot / 2), become (a c - b s, a s + b c) with c, s = cos_t / sin_t[position(t), i].
+ * q [n, nh, hd], k [n, nkv, hd] (either count may be 0) with any strides between tokens and heads; the outputs
+ * may be the inputs themselves (same strides) and must not overlap them otherwise.  positions: NULL (token t is
+ * at t), or [n] int32 / int64; a token whose position is outside the table gets NaN heads. */
+typedef struct cmfc_qk_norm_rope_args {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const float *norm_q, *norm_k; /* [hd] */
+    const float *cos_t, *sin_t;   /* [table_rows, rot / 2] */
+    const void* positions;
+    int64_t q_row, q_head, k_row, k_head, q_out_row, q_out_head, k_out_row, k_out_head;
+    uint64_t n, table_rows;
+    uint32_t nh, nkv, hd, rot;
+    int32_t elem, positions_64, half_split;
+    float eps;
+} cmfc_qk_norm_rope_args;
+int cmfc_qk_norm_rope(int device, const cmfc_qk_norm_rope_args* a, void* stream);
+
+/* Causal attention with a sliding window and first tokens that stay visible, over packed sequences or
+ * caches.  Sequence z has the query rows [q_start[z], q_start[z + 1]) and the k_len[z] key / value rows from
+ * k_start[z] on; its queries are its last positions: query i of Lq stands at p = k_len - Lq + i and sees key j
+ * when j <= p and (p - j < window or j < sinks).  s = scale q.k, with softcap > 0 s = softcap tanh(s / softcap);
+ * out = softmax(s) V; a query that sees no key gets zeros.  Prompts, chunks behind a cache and single tokens are the
+ * same call.  Keys and values that a query does not see never reach its result, whatever they hold.
+ * q, out [q_rows, nh, hd]; k, v [k_rows, nkv, hd], any strides between rows and heads; out must not overlap
+ * the inputs.  q_start [seqs + 1], k_start, k_len [seqs] on the device, ascending q_start; all NULL: one sequence of
+ * all rows (seqs = 1).  Query rows outside every sequence are left as they were.  Offsets are clamped to the
+ * tensors.  window 0: unlimited.  hd <= 256. */
+typedef struct cmfc_window_attention_args {
+    const void *q, *k, *v;
+    void* out;
+    const int32_t *q_start, *k_start, *k_len;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+    uint64_t q_rows, k_rows, window, sinks;
+    uint32_t seqs, nh, nkv, hd;
+    float scale, softcap;
+    int32_t elem;
+} cmfc_window_attention_args;
+int cmfc_window_attention(int device, const cmfc_window_attention_args* a, void* stream);
+
 /* ---- instrumentation ---- */
 /* Exercises the failure path of the bounded device waits (no counterpart in the reference, whose
  * shaders have no waits): launches a one-block kernel that waits, with a budget of `polls` polls
