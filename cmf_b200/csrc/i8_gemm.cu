@@ -51,6 +51,79 @@ __global__ void __launch_bounds__(256) i8_any_kernel(I8Params p) {
         }
 }
 
+// ---- up to 16 tokens: a stream of the weights through the warp-level 8-bit MMA ----
+// Bound: memory, N K bytes of weights.  A block owns 16 weight rows; its 8 warps take 64-byte pieces of k in turn
+// and add their integer sums in shared memory at the end.  Both operands go from global memory straight
+// into MMA fragments: the contraction may run over k in any order as long as both operands use the same one,
+// so a lane loads 16 consecutive levels of its row (and of its token) and they serve two m16n8k32 products.
+// No staging and no barrier in the loop: up to UNROLL x 3 16-byte loads per lane are in flight.
+constexpr int ROWS_WARPS = 8;
+constexpr int ROWS_MAX_TOKENS = 16;
+__device__ __forceinline__ void mma_m16n8k32_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <typename T, int NT>  // NT groups of eight tokens
+__global__ void __launch_bounds__(32 * ROWS_WARPS) i8_rows_kernel(I8Params p) {
+    __shared__ int red[ROWS_WARPS][16][8 * NT + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int8_t* w0 = p.w + min(n0 + g, p.N - 1) * p.ldw + t * 16;       // rows behind the last are read as the last
+    const int8_t* w1 = p.w + min(n0 + g + 8, p.N - 1) * p.ldw + t * 16;   // and not written
+    const int8_t* x[NT];
+    bool live[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        live[i] = i * 8 + g < p.M;
+        x[i] = p.x + (live[i] ? i * 8 + g : 0) * p.ldx + t * 16;
+    }
+    int acc[NT][4] = {};
+    constexpr int UNROLL = 4;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    for (int k0 = warp * 64; k0 < (int)p.K; k0 += ROWS_WARPS * 64 * UNROLL) {
+        uint4 a[UNROLL][2], b[UNROLL][NT];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = k0 + u * ROWS_WARPS * 64;
+            const bool in = k + t * 16 < (int)p.K;  // K is a multiple of 16
+            a[u][0] = in ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : zero;
+            a[u][1] = in ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : zero;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) b[u][i] = in && live[i] ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : zero;
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                mma_m16n8k32_s8(acc[i], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][i].x, b[u][i].y);
+                mma_m16n8k32_s8(acc[i], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][i].z, b[u][i].w);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        red[warp][g][i * 8 + 2 * t] = acc[i][0];
+        red[warp][g][i * 8 + 2 * t + 1] = acc[i][1];
+        red[warp][g + 8][i * 8 + 2 * t] = acc[i][2];
+        red[warp][g + 8][i * 8 + 2 * t + 1] = acc[i][3];
+    }
+    __syncthreads();
+    const int r = threadIdx.x & 15, m = threadIdx.x >> 4;  // 16 tokens in one go
+    if (m < 8 * NT && m < p.M && n0 + r < p.N) {
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < ROWS_WARPS; ++v) sum += red[v][r][m];
+        static_cast<T*>(p.y)[m * p.ldy + n0 + r] = from_f32<T>(i8_scaled(sum, p.x_scale[m], p.w_scale[n0 + r]));
+    }
+}
+
+template <typename T>
+void launch_rows(const I8Params& p, cudaStream_t s) {
+    const unsigned blocks = (unsigned)((p.N + 15) / 16);
+    if (p.M <= 8) i8_rows_kernel<T, 1><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p);
+    else i8_rows_kernel<T, 2><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p);
+}
+
 template <typename T>
 void launch_any(const I8Params& p, cudaStream_t s) {
     i8_any_kernel<T><<<dim3((unsigned)((p.N + GT - 1) / GT), (unsigned)((p.M + GT - 1) / GT)), 256, 0, s>>>(p);
@@ -59,7 +132,15 @@ void launch_any(const I8Params& p, cudaStream_t s) {
 }  // namespace
 
 int launch_i8_matmat(const I8Params& p, int num_sms, cudaStream_t s) {
-    (void)num_sms;
+    const bool aligned = !((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) && p.ldx % 16 == 0 && p.ldw % 16 == 0;
+    if (aligned && p.M <= ROWS_MAX_TOKENS && p.K % 16 == 0) {
+        if (p.out_elem == ET_F32) launch_rows<float>(p, s);
+        else if (p.out_elem == ET_F16) launch_rows<__half>(p, s);
+        else launch_rows<__nv_bfloat16>(p, s);
+        CMFC_CUDA(cudaGetLastError());
+        return OK;
+    }
+    if (aligned) return launch_i8_pair(p, num_sms, s);
     if ((p.M + GT - 1) / GT > 65535) return fail(ERR_UNSUPPORTED, "i8_matmat: too many tokens for rows that are not 16-byte aligned");
     if (p.out_elem == ET_F32) launch_any<float>(p, s);
     else if (p.out_elem == ET_F16) launch_any<__half>(p, s);

@@ -6,6 +6,8 @@ namespace cmfc {
 
 constexpr int64_t I8_MAX_K = 131071;  // 128 * 128 * K stays below 2^31
 
+int launch_i8_pair(const I8Params& p, int num_sms, cudaStream_t s);  // 16-byte aligned rows
+
 #ifdef __CUDACC__
 // The product of the scales is taken first in every kernel, so that all of them round alike.
 __device__ __forceinline__ float i8_scaled(int acc, float x_scale, float w_scale) {

@@ -102,9 +102,11 @@ int i8_matmat_impl(int device, const int8_t* xq, int64_t ldx, const float* xs, c
     p.x_scale = xs;
     p.w_scale = ws;
     p.y = y;
-    p.ldx = b == 1 ? (int64_t)cols : ldx;
-    p.ldw = rows == 1 ? (int64_t)cols : ldw;
-    p.ldy = b == 1 ? (int64_t)rows : ldy;
+    // the pitch of a single row is never used: any that suits the aligned forms will do
+    const auto up16 = [](size_t v) { return (int64_t)((v + 15) / 16 * 16); };
+    p.ldx = b == 1 ? up16(cols) : ldx;
+    p.ldw = rows == 1 ? up16(cols) : ldw;
+    p.ldy = b == 1 ? up16(rows) : ldy;
     p.M = (int64_t)b;
     p.N = (int64_t)rows;
     p.K = (int64_t)cols;
