@@ -392,4 +392,7 @@ int make_tensor_map_2d(CUtensorMap* out, const void* base, int elem_bytes, uint6
 int make_tensor_map_nhwc16(CUtensorMap* out, const void* base, uint64_t channels, uint64_t width, uint64_t height,
                            uint64_t pixel_pitch_bytes, uint32_t box_c, uint32_t box_w, uint32_t box_h, int swizzle);
 
+int make_tensor_map_heads16(CUtensorMap* out, const void* base, uint64_t hd, uint64_t heads, uint64_t rows, uint64_t head_bytes,
+                            uint64_t row_bytes, uint32_t box_c, uint32_t box_heads, uint32_t box_rows);
+
 }  // namespace cmfc

@@ -204,6 +204,7 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             const int nchunks = pl.tt / 32;
             for (int c = ehalf; c < nchunks; c += 2) {
                 uint32_t v[32];
+                __syncwarp();  // the plain stores below leave lanes apart, tcgen05.ld wants the warp together
                 tmem_ld_x32(tmem + lane_addr + a * TT + c * 32, v);
                 tc_wait_ld();
                 if (c + 2 >= nchunks) {  // this warp's last load of the accumulator

@@ -87,6 +87,24 @@ int make_tensor_map_nhwc16(CUtensorMap* out, const void* base, uint64_t channels
     return OK;
 }
 
+// 3-D tiled map over [rows, heads, hd] of 2-byte elements with any strides between rows and heads: dims
+// (hd, heads, rows), box (box_c, box_heads, box_rows), 128-byte swizzle (box_c = 64); what lies out of range reads as zero.
+int make_tensor_map_heads16(CUtensorMap* out, const void* base, uint64_t hd, uint64_t heads, uint64_t rows, uint64_t head_bytes,
+                            uint64_t row_bytes, uint32_t box_c, uint32_t box_heads, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return fail(ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[3] = {hd, heads, rows};
+    cuuint64_t strides[2] = {head_bytes, row_bytes};
+    cuuint32_t box[3] = {box_c, box_heads, box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(ERR_CUDA, "cuTensorMapEncodeTiled (heads) failed with code " + std::to_string((int)r));
+    return OK;
+}
+
 // ---------------- buffers ----------------
 static std::atomic<uint64_t> g_alloc_epoch{1};
 uint64_t alloc_epoch() { return g_alloc_epoch.load(); }

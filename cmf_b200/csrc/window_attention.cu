@@ -202,6 +202,7 @@ int launch_window_any(const WindowAttnParams& p, int elem, cudaStream_t s) {
 
 int launch_window_attention(const WindowAttnParams& p, int elem, int num_sms, cudaStream_t s) {
     (void)num_sms;
+    if (window_prefill_supported(p, elem)) return launch_window_prefill(p, elem, s);
     return launch_window_any(p, elem, s);
 }
 

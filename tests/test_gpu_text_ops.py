@@ -6,6 +6,17 @@ import torch
 from tests import text_ops_ref as ref
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    """After every test: no kernel gave up a bounded wait."""
+    yield
+    from cmf_b200 import gpu
+    torch.cuda.synchronize()
+    gpu.synchronize()
+
+
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
