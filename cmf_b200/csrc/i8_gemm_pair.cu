@@ -196,7 +196,7 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             int tm, tn;
             tile_at(pl, tile, tm, tn);
             const uint32_t a = ti & 1u;
-            if (!mbar_wait<40>(&bars->acc_full[a], (ti >> 1) & 1u, abort_flag, 4)) break;
+            if (!__all_sync(0xffffffffu, mbar_wait<40>(&bars->acc_full[a], (ti >> 1) & 1u, abort_flag, 4))) break;
             tc_fence_after();
             const int row = quarter * 32 + lane;
             const int64_t n = (int64_t)tn * 2 * TW + rank * TW + row;
@@ -252,6 +252,7 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
 
     tc_fence_before();
     __syncthreads();
+    drain_copies(abort_flag);
     cluster.sync();  // the pair's MMAs and signals are done, and with a cut K every slice's sums are written
     if (pl.splits > 1) {
         // one tile per cluster: this CTA finishes the tokens of its slice's share for its 128 weight rows

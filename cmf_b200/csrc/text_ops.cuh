@@ -57,6 +57,12 @@ struct WindowAttnParams {
 int launch_window_attention(const WindowAttnParams& p, int elem, int num_sms, cudaStream_t s);
 
 #ifdef __CUDACC__
+// A kernel that gave up a wait still has copies under way into its shared memory: they get 2 ms (they take
+// microseconds) before the block leaves.
+__device__ __forceinline__ void drain_copies(volatile uint32_t* abort_flag) {
+    if (*abort_flag)
+        for (int i = 0; i < 500; ++i) __nanosleep(4000);
+}
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

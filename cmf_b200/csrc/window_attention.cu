@@ -201,7 +201,8 @@ int launch_window_any(const WindowAttnParams& p, int elem, cudaStream_t s) {
 }
 
 int launch_window_attention(const WindowAttnParams& p, int elem, int num_sms, cudaStream_t s) {
-    (void)num_sms;
+    // up to 32 rows a sequence on average: the key axis is what there is to split
+    if (p.q_rows * (p.nh / p.nkv) <= 32 * (int64_t)p.seqs && window_tokens_supported(p, elem)) return launch_window_tokens(p, elem, num_sms, s);
     if (window_prefill_supported(p, elem)) return launch_window_prefill(p, elem, s);
     return launch_window_any(p, elem, s);
 }

@@ -244,7 +244,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 const bool last_use = !two || x == 1;
                 for (int c = 0; c < NC; ++c) {
                     const uint32_t idx = k_index(j) + c, s = idx % SLOTS;
-                    if (!mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 2)) return false;
+                    if (!__all_sync(0xffffffffu, mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 2))) return false;
                     tc_fence_after();
                     if (leader) {
                         const uint32_t ka = smem_u32(ring + s * SLOT);
@@ -266,7 +266,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 const int live = shift + last_i + 1 - kt.at(j) * KT;
                 for (int c = 0; c < NC; ++c) {
                     const uint32_t idx = v_index(j) + c, s = idx % SLOTS;
-                    if (!mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 3)) return false;
+                    if (!__all_sync(0xffffffffu, mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 3))) return false;
                     if (first_use && live < (c + 1) * VK) {
                         const int r0 = max(0, live - c * VK);
                         const int units = (VK - r0) * 8;  // 16-byte pieces of a group of 64 dims
@@ -290,11 +290,11 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 __syncwarp();
                 return true;
             };
-            bool ok = mbar_wait(&bars->q_full, 0, abort_flag, 4);
+            bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0, abort_flag, 4)) != 0;
             if (ok) ok = issue_s(0);
             if (ok && steps > 1) ok = issue_s(1);
             for (int u = 0; ok && u < steps; ++u) {
-                ok = mbar_wait(&bars->p_full[u & 1], (u >> 1) & 1u, abort_flag, 5);
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[u & 1], (u >> 1) & 1u, abort_flag, 5)) != 0;
                 if (!ok) break;
                 tc_fence_after();
                 ok = issue_o(u);
@@ -316,7 +316,8 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             for (int j = 0; j < n; ++j) {
                 const int x = two ? x0 : (j & 1);
                 const uint32_t ph = (two ? j : j >> 1) & 1u;
-                if (!mbar_wait<20>(&bars->s_full[x], ph, abort_flag, 6)) { ok = false; break; }
+                // the lanes leave a polling loop one by one: tcgen05.ld wants the warp together
+                if (!__all_sync(0xffffffffu, mbar_wait<20>(&bars->s_full[x], ph, abort_flag, 6))) { ok = false; break; }
                 tc_fence_after();
                 uint32_t v[4][32];
 #pragma unroll
@@ -365,7 +366,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     if (j > 0) {
                         // P V of the tile's previous key tile has to be in O (with two query tiles S(j) was issued
                         // behind it, with two S buffers before it); the next one waits for this warp's P
-                        if (!mbar_wait(&bars->o_done[two ? x0 : (j - 1) & 1], (uint32_t)(two ? j - 1 : (j - 1) >> 1) & 1u, abort_flag, 7)) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(&bars->o_done[two ? x0 : (j - 1) & 1], (uint32_t)(two ? j - 1 : (j - 1) >> 1) & 1u, abort_flag, 7))) {
                             ok = false;
                             break;
                         }
@@ -414,7 +415,8 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->p_full[x]);
             }
-            if (n > 0 && ok) ok = mbar_wait(&bars->o_done[two ? x0 : (n - 1) & 1], (uint32_t)(two ? n - 1 : (n - 1) >> 1) & 1u, abort_flag, 8);
+            if (n > 0 && ok)
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[two ? x0 : (n - 1) & 1], (uint32_t)(two ? n - 1 : (n - 1) >> 1) & 1u, abort_flag, 8)) != 0;
             if (ok) {
                 tc_fence_after();
                 const float inv = pos >= 0 ? 1.0f / l : 0.0f;
@@ -455,6 +457,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 
     tc_fence_before();
     __syncthreads();
+    drain_copies(abort_flag);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);

@@ -258,6 +258,18 @@ def test_single_tokens_over_a_cache(nh, nkv, hd, window, sinks, cap, dtype):
     ref.check(out, *ref.window_attention(q, k, v, lens, starts, total, window or 1 << 30, sinks, hd ** -0.5, cap))
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 4, 256), (6, 2, 96), (4, 4, 64)])
+def test_many_single_tokens_over_long_caches(nh, nkv, hd):
+    """Enough blocks and tiles that every ring wraps many times under load; each call gives the first one's bits."""
+    from cmf_b200 import ops
+    prior = [4095 - 61 * i for i in range(48)]
+    q, k, v, starts, total, where = attn_inputs([1] * 48, prior, nh, nkv, hd, torch.bfloat16, slots=4096)
+    first = ops.window_attention(q, k, v, sinks=2, **where)
+    ref.check(first, *ref.window_attention(q, k, v, [1] * 48, starts, total, 1 << 30, 2, hd ** -0.5, 0.0))
+    outs = [ops.window_attention(q, k, v, sinks=2, **where) for _ in range(200)]
+    assert all(torch.equal(o, first) for o in outs)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nh,nkv,hd", [(6, 2, 96), (8, 4, 256), (4, 1, 128)])
 @pytest.mark.parametrize("window,sinks,cap", [(None, 0, 0.0), (150, 4, 0.0), (20, 0, 30.0)])
