@@ -94,6 +94,9 @@ SYMBOLS = {
                                      C.c_void_p, C.c_void_p]),
     "cmfc_i8_matmat": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t,
                                  C.c_size_t, C.c_size_t, C.c_void_p, C.c_int, C.c_int64, C.c_void_p]),
+    "cmfc_i8_linear_workspace": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_size_t, C.c_size_t, C.c_size_t]),
+    "cmfc_i8_linear": (C.c_int, [C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_size_t,
+                                 C.c_size_t, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
     "cmfc_q8_matmat_i8": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p]),
     "cmfc_qk_norm_rope": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p]),
     "cmfc_window_attention": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p]),

@@ -11,7 +11,7 @@
 // 16-byte chunks of a head that hold both members of its pairs (neighbouring chunks, or the same
 // chunk of either half), so the rotation needs no exchange between lanes; a head takes a group of
 // 4 to 32 lanes and a warp works on 32 / group items.
-#include "text_ops.cuh"
+#include "i8_gemm.cuh"
 
 namespace cmfc {
 namespace {
@@ -179,9 +179,6 @@ void norm_rope_typed(const NormRopeParams& p, cudaStream_t s) {
 }
 
 // ---------------- rows to 8 bits ----------------
-// scale = max |x| / 127, q = rint(x / scale) (ties to even), both quotients IEEE f32.  A row of zeros
-// (or one whose scale underflows to zero) gives scale 0 and levels 0; a row that holds an infinity or a
-// NaN gives levels 0 and scale NaN, so that every product with it is NaN.
 // One block per row: the row is read once into registers (CACHED chunks per thread; what does not fit
 // is read again, from L2), so traffic is the input and the levels.
 constexpr int QUANT_THREADS = 256;
@@ -226,25 +223,9 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* _
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < QUANT_THREADS / 32; ++i) top = max(top, red[i]);
-    const bool finite = top < 0x7f800000u;
-    const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __int_as_float(0x7fc00000);
-    const bool zero = !finite || s == 0.0f;
-    if (threadIdx.x == 0) scale[r] = s;
-    // a scale rounded down among the subnormals could let the largest quotient pass 127
-    auto level = [&](float f) { return zero ? 0 : max(-127, min(127, __float2int_rn(__fdiv_rn(f, s)))); };
-    auto put = [&](int64_t c, const float (&o)[V]) {
-        if constexpr (VEC) {
-            uint32_t w[V / 4];
-#pragma unroll
-            for (int e = 0; e < V; e += 4)
-                w[e / 4] = (uint32_t)(uint8_t)level(o[e]) | (uint32_t)(uint8_t)level(o[e + 1]) << 8 |
-                           (uint32_t)(uint8_t)level(o[e + 2]) << 16 | (uint32_t)(uint8_t)level(o[e + 3]) << 24;
-            if constexpr (V == 8) *reinterpret_cast<uint2*>(dst + c * V) = make_uint2(w[0], w[1]);
-            else *reinterpret_cast<uint32_t*>(dst + c * V) = w[0];
-        } else {
-            dst[c] = (int8_t)level(o[0]);
-        }
-    };
+    const RowScale rs(top);
+    if (threadIdx.x == 0) scale[r] = rs.scale;
+    auto put = [&](int64_t c, const float (&o)[V]) { rs.store<V>(dst + c * V, o); };
 #pragma unroll
     for (int i = 0; i < CACHED; ++i) {
         const int64_t c = threadIdx.x + (int64_t)i * QUANT_THREADS;

@@ -4,6 +4,7 @@
 // below and every split of K gives the same bits; one rounding to f32, the product of the two scales, their
 // product, and one rounding to the output type follow.
 #include <atomic>
+#include <type_traits>
 
 #include "i8_gemm.cuh"
 
@@ -64,9 +65,47 @@ __device__ __forceinline__ void mma_m16n8k32_s8(int (&c)[4], uint32_t a0, uint32
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <typename T, int NT>  // NT groups of eight tokens
-__global__ void __launch_bounds__(32 * ROWS_WARPS) i8_rows_kernel(I8Params p) {
+template <typename X>
+__device__ __forceinline__ void round_tokens(const I8Params& p, const X* __restrict__ act, int64_t ld_act, int8_t* levels, float* scales, int* scratch) {
+    constexpr int V = 16 / sizeof(X);
+    const int chunks = (int)(p.K / V), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned* tops = reinterpret_cast<unsigned*>(scratch);  // [tokens][warps]
+    for (int m = 0; m < p.M; ++m) {
+        unsigned top = 0;
+        for (int c = threadIdx.x; c < chunks; c += 32 * ROWS_WARPS) {
+            float v[V];
+            unpack16<X>(__ldg(reinterpret_cast<const uint4*>(act + m * ld_act) + c), v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) tops[m * ROWS_WARPS + warp] = top;
+    }
+    __syncthreads();
+    for (int m = 0; m < p.M; ++m) {
+        unsigned top = 0;
+#pragma unroll
+        for (int w = 0; w < ROWS_WARPS; ++w) top = max(top, tops[m * ROWS_WARPS + w]);
+        const RowScale rs(top);
+        if (threadIdx.x == 0) scales[m] = rs.scale;
+        for (int c = threadIdx.x; c < chunks; c += 32 * ROWS_WARPS) {
+            float v[V];
+            unpack16<X>(__ldg(reinterpret_cast<const uint4*>(act + m * ld_act) + c), v);
+            rs.store<V>(levels + m * (p.K + 16) + c * V, v);
+        }
+    }
+    __syncthreads();
+}
+
+// X is int8_t (levels and scales are there), or the activations' type: then every block rounds the tokens itself first
+// (quantize_rows's arithmetic, level for level), which saves a launch where the tokens are few and short.  The
+// first weights are already on their way meanwhile.
+template <typename T, typename X, int NT>  // NT groups of eight tokens
+__global__ void __launch_bounds__(32 * ROWS_WARPS) i8_rows_kernel(I8Params p, const X* __restrict__ act, int64_t ld_act) {
+    constexpr bool FUSED = !std::is_same<X, int8_t>::value;
+    extern __shared__ __align__(16) int8_t levels[];  // FUSED: [tokens][K + 16], rows shifted by 16 bytes
     __shared__ int red[ROWS_WARPS][16][8 * NT + 1];
+    __shared__ float scales[FUSED ? 8 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t n0 = (int64_t)blockIdx.x * 16;
     const int8_t* w0 = p.w + min(n0 + g, p.N - 1) * p.ldw + t * 16;       // rows behind the last are read as the last
@@ -76,21 +115,35 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) i8_rows_kernel(I8Params p) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         live[i] = i * 8 + g < p.M;
-        x[i] = p.x + (live[i] ? i * 8 + g : 0) * p.ldx + t * 16;
+        if constexpr (FUSED) x[i] = levels + (live[i] ? i * 8 + g : 0) * (p.K + 16) + t * 16;
+        else x[i] = p.x + (live[i] ? i * 8 + g : 0) * p.ldx + t * 16;
     }
     int acc[NT][4] = {};
     constexpr int UNROLL = 4;
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    for (int k0 = warp * 64; k0 < (int)p.K; k0 += ROWS_WARPS * 64 * UNROLL) {
-        uint4 a[UNROLL][2], b[UNROLL][NT];
+    uint4 a[UNROLL][2], b[UNROLL][NT];
+    auto load_w = [&](int k0) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int k = k0 + u * ROWS_WARPS * 64;
             const bool in = k + t * 16 < (int)p.K;  // K is a multiple of 16
             a[u][0] = in ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : zero;
             a[u][1] = in ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : zero;
+        }
+    };
+    load_w(warp * 64);
+    if constexpr (FUSED) round_tokens<X>(p, act, ld_act, levels, scales, &red[0][0][0]);
+    for (int k0 = warp * 64; k0 < (int)p.K; k0 += ROWS_WARPS * 64 * UNROLL) {
+        if (k0 != warp * 64) load_w(k0);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) b[u][i] = in && live[i] ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : zero;
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = k0 + u * ROWS_WARPS * 64;
+            const bool in = k + t * 16 < (int)p.K;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                if constexpr (FUSED) b[u][i] = in && live[i] ? *reinterpret_cast<const uint4*>(x[i] + k) : zero;
+                else b[u][i] = in && live[i] ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : zero;
+            }
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
@@ -113,15 +166,28 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) i8_rows_kernel(I8Params p) {
         int sum = 0;
 #pragma unroll
         for (int v = 0; v < ROWS_WARPS; ++v) sum += red[v][r][m];
-        static_cast<T*>(p.y)[m * p.ldy + n0 + r] = from_f32<T>(i8_scaled(sum, p.x_scale[m], p.w_scale[n0 + r]));
+        static_cast<T*>(p.y)[m * p.ldy + n0 + r] = from_f32<T>(i8_scaled(sum, FUSED ? scales[FUSED ? m : 0] : p.x_scale[m], p.w_scale[n0 + r]));
     }
 }
 
 template <typename T>
 void launch_rows(const I8Params& p, cudaStream_t s) {
     const unsigned blocks = (unsigned)((p.N + 15) / 16);
-    if (p.M <= 8) i8_rows_kernel<T, 1><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p);
-    else i8_rows_kernel<T, 2><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p);
+    if (p.M <= 8) i8_rows_kernel<T, int8_t, 1><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p, nullptr, 0);
+    else i8_rows_kernel<T, int8_t, 2><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p, nullptr, 0);
+}
+
+template <typename T, typename X>
+int launch_fused(const I8Params& p, const void* act, int64_t ld_act, cudaStream_t s) {
+    i8_rows_kernel<T, X, 1><<<(unsigned)((p.N + 15) / 16), 32 * ROWS_WARPS, (size_t)(p.M * (p.K + 16)), s>>>(p, static_cast<const X*>(act), ld_act);
+    CMFC_CUDA(cudaGetLastError());
+    return OK;
+}
+template <typename T>
+int launch_fused_x(const I8Params& p, const void* act, int elem, int64_t ld_act, cudaStream_t s) {
+    if (elem == ET_F32) return launch_fused<T, float>(p, act, ld_act, s);
+    if (elem == ET_F16) return launch_fused<T, __half>(p, act, ld_act, s);
+    return launch_fused<T, __nv_bfloat16>(p, act, ld_act, s);
 }
 
 template <typename T>
@@ -130,6 +196,18 @@ void launch_any(const I8Params& p, cudaStream_t s) {
 }
 
 }  // namespace
+
+// Rounding inside the product: every block of 16 weight rows does it again, from L2, for all tokens.
+bool i8_fused_fits(int64_t M, int64_t K) { return M <= 8 && M * K <= 32768 && K % 16 == 0; }
+bool i8_fused_supported(const I8Params& p, const void* act, int elem, int64_t ld_act) {
+    return i8_fused_fits(p.M, p.K) && !((reinterpret_cast<uintptr_t>(act) | reinterpret_cast<uintptr_t>(p.w)) & 15) && p.ldw % 16 == 0 &&
+           (ld_act * (int64_t)elem_bytes(elem)) % 16 == 0;
+}
+int launch_i8_fused(const I8Params& p, const void* act, int elem, int64_t ld_act, cudaStream_t s) {
+    if (p.out_elem == ET_F32) return launch_fused_x<float>(p, act, elem, ld_act, s);
+    if (p.out_elem == ET_F16) return launch_fused_x<__half>(p, act, elem, ld_act, s);
+    return launch_fused_x<__nv_bfloat16>(p, act, elem, ld_act, s);
+}
 
 int launch_i8_matmat(const I8Params& p, int num_sms, cudaStream_t s) {
     const bool aligned = !((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) && p.ldx % 16 == 0 && p.ldw % 16 == 0;

@@ -83,6 +83,24 @@ int quantize_rows_impl(int device, const void* x, int elem, size_t rows, size_t 
     return OK;
 }
 
+int64_t up16(size_t v) { return (int64_t)((v + 15) / 16 * 16); }
+// the pitch of a single row is never used: any that suits the aligned forms will do
+int64_t pitch(size_t rows, size_t cols, int64_t ld) { return rows == 1 ? up16(cols) : ld; }
+
+I8Params i8_params(const int8_t* wq, int64_t ldw, const float* ws, size_t b, size_t rows, size_t cols, void* y, int elem, int64_t ldy) {
+    I8Params p = {};
+    p.w = wq;
+    p.w_scale = ws;
+    p.y = y;
+    p.ldw = pitch(rows, cols, ldw);
+    p.ldy = pitch(b, rows, ldy);
+    p.M = (int64_t)b;
+    p.N = (int64_t)rows;
+    p.K = (int64_t)cols;
+    p.out_elem = elem;
+    return p;
+}
+
 int i8_matmat_impl(int device, const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw, const float* ws,
                    size_t b, size_t rows, size_t cols, void* y, int elem, int64_t ldy, cudaStream_t s) {
     NEED(elem_ok(elem), "i8_matmat: unknown output type");
@@ -96,24 +114,53 @@ int i8_matmat_impl(int device, const int8_t* xq, int64_t ldx, const float* xs, c
          "i8_matmat: a row pitch is shorter than a row");
     OnDevice on;
     CMFC_TRY(on.enter(device, s));
-    I8Params p;
+    I8Params p = i8_params(wq, ldw, ws, b, rows, cols, y, elem, ldy);
     p.x = xq;
-    p.w = wq;
     p.x_scale = xs;
-    p.w_scale = ws;
-    p.y = y;
-    // the pitch of a single row is never used: any that suits the aligned forms will do
-    const auto up16 = [](size_t v) { return (int64_t)((v + 15) / 16 * 16); };
-    p.ldx = b == 1 ? up16(cols) : ldx;
-    p.ldw = rows == 1 ? up16(cols) : ldw;
-    p.ldy = b == 1 ? up16(rows) : ldy;
-    p.M = (int64_t)b;
-    p.N = (int64_t)rows;
-    p.K = (int64_t)cols;
-    p.out_elem = elem;
+    p.ldx = pitch(b, cols, ldx);
     p.status = on.c->status;
     CMFC_TRY(launch_i8_matmat(p, on.c->num_sms, s));
     count_launches(on.c, 1);
+    return OK;
+}
+
+size_t i8_linear_workspace(const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, size_t b, size_t rows, size_t cols) {
+    if (b > INT_MAX || cols > (size_t)I8_MAX_K || rows > INT_MAX || !elem_ok(elem)) return 0;  // refused by the call itself
+    const I8Params p = i8_params(wq, ldw, nullptr, b, rows, cols, nullptr, ET_F32, (int64_t)rows);
+    return i8_fused_supported(p, x, elem, pitch(b, cols, ldx)) ? 0 : b * (size_t)up16(cols) + 4 * b;
+}
+
+int i8_linear_impl(int device, const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, const float* ws, size_t b,
+                   size_t rows, size_t cols, void* y, int y_elem, int64_t ldy, void* work, size_t work_bytes, cudaStream_t s) {
+    NEED(elem_ok(elem) && elem_ok(y_elem), "i8_linear: unknown element type");
+    NEED(b <= INT_MAX && rows >= 1 && rows <= INT_MAX, "i8_linear: b must be below 2^31, rows in [1, 2^31)");
+    NEED(cols >= 1, "i8_linear: cols must not be 0");
+    if (cols > (size_t)I8_MAX_K) return fail(ERR_UNSUPPORTED, "i8_linear: cols above 131071 could overflow the 32-bit sum");
+    if (b == 0) return OK;
+    NEED(x && wq && ws && y, "i8_linear: null pointer");
+    NEED(stride_ok(ldx) && stride_ok(ldw) && stride_ok(ldy), "i8_linear: bad row pitch");
+    NEED((b == 1 || ldx >= (int64_t)cols) && (rows == 1 || ldw >= (int64_t)cols) && (b == 1 || ldy >= (int64_t)rows),
+         "i8_linear: a row pitch is shorter than a row");
+    OnDevice on;
+    CMFC_TRY(on.enter(device, s));
+    I8Params p = i8_params(wq, ldw, ws, b, rows, cols, y, y_elem, ldy);
+    p.status = on.c->status;
+    if (i8_fused_supported(p, x, elem, pitch(b, cols, ldx))) {
+        CMFC_TRY(launch_i8_fused(p, x, elem, pitch(b, cols, ldx), s));
+        count_launches(on.c, 1);
+        return OK;
+    }
+    const size_t levels = b * (size_t)up16(cols);
+    NEED(work && !(reinterpret_cast<uintptr_t>(work) & 15) && work_bytes >= levels + 4 * b,
+         "i8_linear: this call needs a 16-byte aligned workspace of cmfc_i8_linear_workspace() bytes");
+    int8_t* q = static_cast<int8_t*>(work);
+    float* scale = reinterpret_cast<float*>(q + levels);
+    CMFC_TRY(launch_quantize_rows(x, elem, p.M, p.K, ldx, q, up16(cols), scale, s));
+    p.x = q;
+    p.x_scale = scale;
+    p.ldx = up16(cols);
+    CMFC_TRY(launch_i8_matmat(p, on.c->num_sms, s));
+    count_launches(on.c, 2);
     return OK;
 }
 
@@ -214,6 +261,19 @@ extern "C" int cmfc_i8_matmat(int device, const int8_t* xq, int64_t ldx, const f
                               void* stream) {
     return guarded([&] {
         return i8_matmat_impl(device, xq, ldx, x_scale, wq, ldw, w_scale, b, rows, cols, y, elem, ldy, (cudaStream_t)stream);
+    });
+}
+
+extern "C" size_t cmfc_i8_linear_workspace(const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, size_t b,
+                                           size_t rows, size_t cols) {
+    return i8_linear_workspace(x, elem, ldx, wq, ldw, b, rows, cols);
+}
+
+extern "C" int cmfc_i8_linear(int device, const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, const float* w_scale,
+                              size_t b, size_t rows, size_t cols, void* y, int y_elem, int64_t ldy, void* work, size_t work_bytes,
+                              void* stream) {
+    return guarded([&] {
+        return i8_linear_impl(device, x, elem, ldx, wq, ldw, w_scale, b, rows, cols, y, y_elem, ldy, work, work_bytes, (cudaStream_t)stream);
     });
 }
 

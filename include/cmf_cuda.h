@@ -297,6 +297,13 @@ int cmfc_quantize_rows(int device, const void* x, int elem, size_t rows, size_t 
  * (cols <= 131071).  Fastest with pitches and bases that are multiples of 16 bytes. */
 int cmfc_i8_matmat(int device, const int8_t* xq, int64_t ldx, const float* x_scale, const int8_t* wq, int64_t ldw,
                    const float* w_scale, size_t b, size_t rows, size_t cols, void* y, int elem, int64_t ldy, void* stream);
+/* The two in one call: x [b, cols] of type `elem` through 8-bit weights, the same bits as cmfc_quantize_rows and
+ * cmfc_i8_matmat one after the other.  `work` is the caller's: cmfc_i8_linear_workspace() bytes, 16-byte aligned, free to
+ * use again when the stream has passed the call.  That is 0 (and work may be NULL) for a few short tokens, whose
+ * rounding the product does itself. */
+size_t cmfc_i8_linear_workspace(const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, size_t b, size_t rows, size_t cols);
+int cmfc_i8_linear(int device, const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, const float* w_scale,
+                   size_t b, size_t rows, size_t cols, void* y, int y_elem, int64_t ldy, void* work, size_t work_bytes, void* stream);
 /* cmfc_q8_matmat (gpu.rs:1155) with the activations rounded to 8 bits too (cmfc_quantize_rows): host f32
  * in and out; tensor idx must be q8_row.  Runs on the library's stream and returns when done. */
 int cmfc_q8_matmat_i8(cmfc_model* m, int64_t idx, const float* xs, size_t b, size_t rows, size_t cols, float* out);

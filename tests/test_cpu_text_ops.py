@@ -85,6 +85,11 @@ def test_products_refuse():
     refused(-3, ops.i8_matmat, xq, xs, w, s, out=torch.zeros(4, 9))
     refused(-2, ops.i8_matmat, xq, xs, w, s, out_dtype=torch.float64)
     refused(-1, ops.i8_linear, x, w, s)
+    refused(-3, ops.i8_linear, x, w[:, :16], s)
+    refused(-2, ops.i8_linear, x, x, s)
+    refused(-2, ops.i8_linear, x.int(), w, s)
+    refused(-3, ops.i8_linear, x, w, s, out=torch.zeros(8, 4))
+    refused(-3, ops.i8_linear, x, w, s, out_dtype=torch.float32, out=torch.zeros(4, 8, dtype=torch.float16))
 
 
 def test_library_refuses_before_any_device_call():
@@ -128,4 +133,14 @@ def test_library_refuses_before_any_device_call():
     assert m(elem=9) == -1 and m(rows=0) == -1 and m(cols=0) == -1 and m(w=None) == -1 and m(ldx=7) == -1 and m(ldy=3) == -1
     assert m(cols=131072, ldx=131072, ldw=131072) == -2
     assert m(b=0) == 0
+    # the workspace of i8_linear: none for a few short aligned tokens, levels and scales otherwise
+    assert L.cmfc_i8_linear_workspace(p, 2, 64, p, 64, 1, 8, 64) == 0
+    assert L.cmfc_i8_linear_workspace(p, 2, 64, p, 64, 9, 8, 64) == 9 * 64 + 36
+    assert L.cmfc_i8_linear_workspace(C.c_void_p(258), 2, 64, p, 64, 2, 8, 64) == 2 * 64 + 8
+    assert L.cmfc_i8_linear_workspace(p, 2, 33, p, 33, 2, 8, 33) == 2 * 48 + 8
+    li = lambda **kw: L.cmfc_i8_linear(*{**dict(dev=0, x=p, elem=0, ldx=8, w=p, ldw=8, ws=p, b=4, rows=4, cols=8, y=p, ye=0, ldy=4, work=p, nb=100,  # noqa: E731
+                                                st=None), **kw}.values())
+    assert li(elem=9) == -1 and li(ye=9) == -1 and li(rows=0) == -1 and li(cols=0) == -1 and li(x=None) == -1 and li(ldx=7) == -1 and li(ldy=3) == -1
+    assert li(cols=131072, ldx=131072, ldw=131072) == -2
+    assert li(b=0) == 0
     assert L.cmfc_q8_matmat_i8(None, 0, p, 1, 1, 1, p) == -1

@@ -522,7 +522,33 @@ def test_the_status_word_is_clear_and_launches_are_counted():
     from cmf_b200 import gpu, ops
     gpu.set_current_device(0)
     before = gpu.launch_count()
-    ops.i8_linear(torch.ones(2, 64, device="cuda"), torch.ones(16, 64, dtype=torch.int8, device="cuda"), torch.ones(16, device="cuda"))
+    w, s = torch.ones(16, 64, dtype=torch.int8, device="cuda"), torch.ones(16, device="cuda")
+    ops.i8_matmat(*ops.quantize_rows(torch.ones(2, 64, device="cuda")), w, s)
     torch.cuda.synchronize()
     gpu.synchronize()                       # no kernel gave up a wait
     assert gpu.launch_count() == before + 2
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,rows,cols", [(1, 2304, 2304), (1, 40, 16), (3, 130, 4096), (8, 300, 4096), (8, 64, 4112), (9, 64, 512), (4, 33, 100), (1, 7, 33), (300, 520, 272)])
+def test_i8_linear_is_the_two_operators_in_one(b, rows, cols, dtype):
+    """Bit for bit, whether the product rounds the tokens itself or not; rows off the 16-byte boundary too."""
+    from cmf_b200 import ops
+    g = gen(b + rows)
+    wide = randn(g, b, cols + 9, dtype=dtype)
+    wide[0, cols // 2] = 40.0
+    w = torch.randint(-128, 128, (rows, cols + 16), generator=g, device="cuda", dtype=torch.int8)
+    s = torch.rand(rows, generator=g, device="cuda") * 1e-2
+    for x, wq in ((wide[:, :cols].contiguous(), w[:, :cols].contiguous()), (wide[:, 1:1 + cols], w[:, :cols]), (wide[:, :cols].contiguous(), w[:, 3:3 + cols])):
+        for out in TYPES:
+            want = ops.i8_matmat(*ops.quantize_rows(x), wq, s, out_dtype=out)
+            assert torch.equal(ops.i8_linear(x, wq, s, out_dtype=out), want)
+            canvas = torch.full((b, rows + 5), 3.0, dtype=out, device="cuda")
+            ops.i8_linear(x, wq, s, out=canvas[:, 2:2 + rows])
+            assert torch.equal(canvas[:, 2:2 + rows], want) and (canvas[:, :2] == 3.0).all() and (canvas[:, 2 + rows:] == 3.0).all()
+    assert ops.i8_linear(x, wq, s).dtype == dtype
+    bad = wide[:, :cols].contiguous()
+    bad[b - 1, 0] = float("inf")
+    y = ops.i8_linear(bad, w[:, :cols].contiguous(), s)
+    assert torch.isnan(y[b - 1]).all() and torch.isfinite(y[:b - 1].float()).all()
+    assert (ops.i8_linear(torch.zeros_like(bad), w[:, :cols].contiguous(), s) == 0).all()
