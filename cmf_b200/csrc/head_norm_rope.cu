@@ -179,45 +179,83 @@ void norm_rope_typed(const NormRopeParams& p, cudaStream_t s) {
 }
 
 // ---------------- rows to 8 bits ----------------
-// One block per row: the row is read once into registers (CACHED chunks per thread; what does not fit
-// is read again, from L2), so traffic is the input and the levels.
+// Bound: memory, the activations once and the levels once.  A row is read once into registers by a warp (short rows)
+// or a block of 256 threads, CH 16-byte chunks a thread; what does not fit is read again, from L2.
 constexpr int QUANT_THREADS = 256;
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t cols,
-                                                                      int8_t* __restrict__ q, int64_t ldq,
-                                                                      float* __restrict__ scale) {
-    constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-    constexpr int CACHED = VEC ? 4 : 8;
+// top of the bit patterns of |x| over a chunk, NaN above infinity above every number; 16-bit types two at a time
+template <typename T>
+__device__ __forceinline__ void chunk_top(const uint4& r, unsigned& top) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) top = max(top, w[i] & 0x7fffffffu);
+        else top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    }
+}
+// ... and what chunk_top() left as the f32 bit pattern
+template <typename T>
+__device__ __forceinline__ unsigned top_f32(unsigned top) {
+    if constexpr (sizeof(T) == 4) {
+        return top;
+    } else {
+        top = max(top & 0xffffu, top >> 16);
+        const unsigned short h = (unsigned short)top;
+        return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&h))) & 0x7fffffffu;
+    }
+}
+
+// TPR threads per row (32 or 256), CH chunks kept by each
+template <typename T, int TPR, int CH>
+__global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int rows, int chunks,
+                                                                      int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int64_t r = (int64_t)blockIdx.x * (QUANT_THREADS / TPR) + threadIdx.x / TPR;
+    if (TPR == 32 && r >= rows) return;  // a whole warp
+    const int t = threadIdx.x % TPR;
+    const uint4* src = reinterpret_cast<const uint4*>(x + r * ldx);
+    int8_t* dst = q + r * ldq;
+    uint4 raw[CH];
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) raw[i] = t + i * TPR < chunks ? __ldg(src + t + i * TPR) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) chunk_top<T>(raw[i], top);
+    for (int c = t + CH * TPR; c < chunks; c += TPR) chunk_top<T>(__ldg(src + c), top);
+    top = __reduce_max_sync(0xffffffffu, top_f32<T>(top));
+    if constexpr (TPR > 32) {
+        __shared__ unsigned red[TPR / 32];
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TPR / 32; ++i) top = max(top, red[i]);
+    }
+    const RowScale rs(top);
+    if (t == 0) scale[r] = rs.scale;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+        if (t + i * TPR < chunks) {
+            float v[V];
+            unpack16<T>(raw[i], v);
+            rs.store<V>(dst + (t + i * TPR) * V, v);
+        }
+    for (int c = t + CH * TPR; c < chunks; c += TPR) {
+        float v[V];
+        unpack16<T>(__ldg(src + c), v);
+        rs.store<V>(dst + c * V, v);
+    }
+}
+
+// rows of any length, pitch and alignment, value by value
+template <typename T>
+__global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_any_kernel(const T* __restrict__ x, int64_t ldx, int cols, int8_t* __restrict__ q,
+                                                                          int64_t ldq, float* __restrict__ scale) {
     const int64_t r = blockIdx.x;
     const T* src = x + r * ldx;
     int8_t* dst = q + r * ldq;
-    const int64_t chunks = cols / V;
     __shared__ unsigned red[QUANT_THREADS / 32];
-    float v[CACHED][V];
-    unsigned top = 0;  // of the bit patterns of |x|: NaN above infinity above every number
-    auto fetch = [&](int64_t c, float (&o)[V]) {
-        if constexpr (VEC) unpack16<T>(*reinterpret_cast<const uint4*>(src + c * V), o);
-        else o[0] = to_f32(src[c]);
-    };
-#pragma unroll
-    for (int i = 0; i < CACHED; ++i) {
-        const int64_t c = threadIdx.x + (int64_t)i * QUANT_THREADS;
-        if (c < chunks) {
-            fetch(c, v[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[i][e] = 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
-    }
-    for (int64_t c = threadIdx.x + (int64_t)CACHED * QUANT_THREADS; c < chunks; c += QUANT_THREADS) {
-        float o[V];
-        fetch(c, o);
-#pragma unroll
-        for (int e = 0; e < V; ++e) top = max(top, __float_as_uint(o[e]) & 0x7fffffffu);
-    }
+    unsigned top = 0;
+    for (int c = threadIdx.x; c < cols; c += QUANT_THREADS) top = max(top, __float_as_uint(to_f32(src[c])) & 0x7fffffffu);
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
@@ -225,16 +263,9 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* _
     for (int i = 0; i < QUANT_THREADS / 32; ++i) top = max(top, red[i]);
     const RowScale rs(top);
     if (threadIdx.x == 0) scale[r] = rs.scale;
-    auto put = [&](int64_t c, const float (&o)[V]) { rs.store<V>(dst + c * V, o); };
-#pragma unroll
-    for (int i = 0; i < CACHED; ++i) {
-        const int64_t c = threadIdx.x + (int64_t)i * QUANT_THREADS;
-        if (c < chunks) put(c, v[i]);
-    }
-    for (int64_t c = threadIdx.x + (int64_t)CACHED * QUANT_THREADS; c < chunks; c += QUANT_THREADS) {
-        float o[V];
-        fetch(c, o);
-        put(c, o);
+    for (int c = threadIdx.x; c < cols; c += QUANT_THREADS) {
+        const float v = to_f32(src[c]);
+        rs.store<1>(dst + c, &v);
     }
 }
 
@@ -243,8 +274,20 @@ void quantize_rows_typed(const void* x, int64_t rows, int64_t cols, int64_t ldx,
     constexpr int V = 16 / sizeof(T);
     const bool vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !(reinterpret_cast<uintptr_t>(q) & 7) && cols % V == 0 && ldx % V == 0 && ldq % V == 0;
     const T* xt = static_cast<const T*>(x);
-    if (vec) quantize_rows_kernel<T, true><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, cols, q, ldq, scale);
-    else quantize_rows_kernel<T, false><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, cols, q, ldq, scale);
+    const int chunks = (int)(cols / V);
+    if (!vec) {
+        quantize_rows_any_kernel<T><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, (int)cols, q, ldq, scale);
+    } else if (chunks <= 32 * 16 && rows >= 512) {
+        // a warp per row keeps up to 16 chunks in registers and needs no block barrier; with few rows a block per
+        // row spreads them over more SMs
+        const unsigned blocks = (unsigned)((rows + 7) / 8);
+        if (chunks <= 32 * 8) quantize_rows_kernel<T, 32, 8><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+        else quantize_rows_kernel<T, 32, 16><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+    } else if (chunks <= 256 * 2) {
+        quantize_rows_kernel<T, 256, 2><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+    } else {
+        quantize_rows_kernel<T, 256, 8><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+    }
 }
 
 }  // namespace

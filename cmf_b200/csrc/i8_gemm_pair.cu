@@ -258,23 +258,44 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         // one tile per cluster: this CTA finishes the tokens of its slice's share for its 128 weight rows
         int tm, tn;
         tile_at(pl, unit, tm, tn);
-        const int row = threadIdx.x % TW, sub = threadIdx.x / TW, subs = THREADS / TW;
+        // (four rows a thread, four tokens in flight: the remote loads are what takes time here)
+        const int row = lane * 4;
         const int64_t n = (int64_t)tn * 2 * TW + rank * TW + row;
         const int t0 = slice * pl.tt / pl.splits, t1 = (slice + 1) * pl.tt / pl.splits;
-        const int* part[MAX_SPLITS];
+        const int4* part[MAX_SPLITS];
 #pragma unroll
         for (int s = 0; s < MAX_SPLITS; ++s)
-            part[s] = static_cast<const int*>(cluster.map_shared_rank(static_cast<void*>(smem), (unsigned)(2 * (s < pl.splits ? s : 0) + rank)));
-        if (sub < subs && n < p.N) {
-            const float ws = p.w_scale[n];
-            for (int t = t0 + sub; t < t1; t += subs) {
-                const int64_t m = (int64_t)tm * pl.tt + t;
-                if (m >= p.M) break;
-                int acc = 0;
+            part[s] = static_cast<const int4*>(cluster.map_shared_rank(static_cast<void*>(smem), (unsigned)(2 * (s < pl.splits ? s : 0) + rank))) + lane;
+        float ws[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ws[e] = n + e < p.N ? p.w_scale[n + e] : 0.0f;
+        constexpr int FLY = 4;
+        for (int tb = t0 + warp; tb < t1; tb += FLY * (THREADS / 32)) {
+            int4 acc[FLY];
+#pragma unroll
+            for (int f = 0; f < FLY; ++f) {
+                const int t = tb + f * (THREADS / 32);
+                acc[f] = make_int4(0, 0, 0, 0);
 #pragma unroll
                 for (int s = 0; s < MAX_SPLITS; ++s)
-                    if (s < pl.splits) acc += part[s][t * TW + row];
-                store_one<T>(p, m, n, acc, p.x_scale[m], ws);
+                    if (s < pl.splits && t < t1) {
+                        const int4 v = part[s][t * (TW / 4)];
+                        acc[f].x += v.x;
+                        acc[f].y += v.y;
+                        acc[f].z += v.z;
+                        acc[f].w += v.w;
+                    }
+            }
+#pragma unroll
+            for (int f = 0; f < FLY; ++f) {
+                const int t = tb + f * (THREADS / 32);
+                const int64_t m = (int64_t)tm * pl.tt + t;
+                if (t >= t1 || m >= p.M) continue;
+                const float xs = p.x_scale[m];
+                const int a[4] = {acc[f].x, acc[f].y, acc[f].z, acc[f].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < p.N) store_one<T>(p, m, n + e, a[e], xs, ws[e]);
             }
         }
         cluster.sync();  // nobody's shared memory goes away while another CTA reads it
