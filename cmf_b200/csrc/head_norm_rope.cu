@@ -234,16 +234,8 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* _
     if (t == 0) scale[r] = rs.scale;
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-        if (t + i * TPR < chunks) {
-            float v[V];
-            unpack16<T>(raw[i], v);
-            rs.store<V>(dst + (t + i * TPR) * V, v);
-        }
-    for (int c = t + CH * TPR; c < chunks; c += TPR) {
-        float v[V];
-        unpack16<T>(__ldg(src + c), v);
-        rs.store<V>(dst + c * V, v);
-    }
+        if (t + i * TPR < chunks) rs.store<T>(dst + (t + i * TPR) * V, raw[i]);
+    for (int c = t + CH * TPR; c < chunks; c += TPR) rs.store<T>(dst + c * V, __ldg(src + c));
 }
 
 // rows of any length, pitch and alignment, value by value
@@ -263,10 +255,7 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_any_kernel(const 
     for (int i = 0; i < QUANT_THREADS / 32; ++i) top = max(top, red[i]);
     const RowScale rs(top);
     if (threadIdx.x == 0) scale[r] = rs.scale;
-    for (int c = threadIdx.x; c < cols; c += QUANT_THREADS) {
-        const float v = to_f32(src[c]);
-        rs.store<1>(dst + c, &v);
-    }
+    for (int c = threadIdx.x; c < cols; c += QUANT_THREADS) dst[c] = rs.level(to_f32(src[c]));
 }
 
 template <typename T>
@@ -281,10 +270,14 @@ void quantize_rows_typed(const void* x, int64_t rows, int64_t cols, int64_t ldx,
         // a warp per row keeps up to 16 chunks in registers and needs no block barrier; with few rows a block per
         // row spreads them over more SMs
         const unsigned blocks = (unsigned)((rows + 7) / 8);
-        if (chunks <= 32 * 8) quantize_rows_kernel<T, 32, 8><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+        if (chunks <= 32 * 4) quantize_rows_kernel<T, 32, 4><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+        else if (chunks <= 32 * 8) quantize_rows_kernel<T, 32, 8><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+        else if (chunks <= 32 * 12) quantize_rows_kernel<T, 32, 12><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
         else quantize_rows_kernel<T, 32, 16><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
     } else if (chunks <= 256 * 2) {
         quantize_rows_kernel<T, 256, 2><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
+    } else if (chunks <= 256 * 4) {
+        quantize_rows_kernel<T, 256, 4><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
     } else {
         quantize_rows_kernel<T, 256, 8><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
     }

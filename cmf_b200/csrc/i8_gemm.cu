@@ -89,9 +89,7 @@ __device__ __forceinline__ void round_tokens(const I8Params& p, const X* __restr
         const RowScale rs(top);
         if (threadIdx.x == 0) scales[m] = rs.scale;
         for (int c = threadIdx.x; c < chunks; c += 32 * ROWS_WARPS) {
-            float v[V];
-            unpack16<X>(__ldg(reinterpret_cast<const uint4*>(act + m * ld_act) + c), v);
-            rs.store<V>(levels + m * (p.K + 16) + c * V, v);
+            rs.store<X>(levels + m * (p.K + 16) + c * V, __ldg(reinterpret_cast<const uint4*>(act + m * ld_act) + c));
         }
     }
     __syncthreads();

@@ -27,41 +27,71 @@ struct RowScale {
         inv = __frcp_rn(scale);
     }
     // the definition; a scale rounded down among the subnormals could let the largest quotient pass 127
-    __device__ __forceinline__ int exact(float f) const { return zero ? 0 : max(-127, min(127, __float2int_rn(__fdiv_rn(f, scale)))); }
-    // Levels without a division each: t = f * (1 / scale) is off f / scale by at most 127 x 2 x 2^-24 = 1.6e-5 (two
-    // roundings of a number up to 127), and the rounded quotient by at most 127 x 2^-24 = 7.6e-6, so both round to the same
-    // integer unless t lies within 2.4e-5 of a half.  Values that do (one in some thousands) take the definition.
-    // Rounding to an integer is the addition of 1.5 x 2^23; its low byte is the level.
-    template <int V>
-    __device__ __forceinline__ void levels(const float* v, uint32_t* bits) const {
-        constexpr float MAGIC = 12582912.0f;
-        float far = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float t = v[e] * inv, u = t + MAGIC;
-            bits[e] = __float_as_uint(u);
-            far = fmaxf(far, fabsf(t - (u - MAGIC)));
-        }
-        if (slow || zero || far > 0.49997f) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) bits[e] = (uint32_t)exact(v[e]);
-        }
+    static __device__ __forceinline__ int exact(float f, float scale, bool zero) {
+        return zero ? 0 : max(-127, min(127, __float2int_rn(__fdiv_rn(f, scale))));
     }
-    // V (1, 4 or 8) levels to an address aligned to V
-    template <int V>
-    __device__ __forceinline__ void store(int8_t* dst, const float* v) const {
-        uint32_t b[V];
-        levels<V>(v, b);
-        if constexpr (V == 1) {
-            *dst = (int8_t)b[0];
-        } else {
-            uint32_t w[V / 4];
+    __device__ __forceinline__ int8_t level(float f) const { return (int8_t)exact(f, scale, zero); }
+    // a 16-byte chunk of T -> its levels, one byte each (.y stays 0 for the four of f32)
+    template <typename T>
+    static __device__ __noinline__ uint2 exact_chunk(uint4 raw, float scale, bool zero) {
+        constexpr int V = 16 / (int)sizeof(T);
+        float v[V];
+        unpack16<T>(raw, v);
+        uint32_t w[2] = {0u, 0u};
 #pragma unroll
-            for (int e = 0; e < V; e += 4)
-                w[e / 4] = __byte_perm(__byte_perm(b[e], b[e + 1], 0x0040), __byte_perm(b[e + 2], b[e + 3], 0x0040), 0x5410);
-            if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-            else *reinterpret_cast<uint32_t*>(dst) = w[0];
+        for (int e = 0; e < V; ++e) w[e / 4] |= (uint32_t)(uint8_t)exact(v[e], scale, zero) << (8 * (e & 3));
+        return make_uint2(w[0], w[1]);
+    }
+    // The same without a division each.  t = RN(f * inv) is off f / scale by at most 127 x 2 x 2^-24 = 1.6e-5 (two roundings
+    // of a number up to 127), and the rounded quotient by at most 127 x 2^-24 = 7.6e-6, so both round to the same integer
+    // unless t lies within 2.4e-5 of a half h (bf16 values over a bf16 maximum do in 0.3 % of all cases).  There the
+    // remainder e = f - h scale is exact: h has 8 bits, so e is a multiple of half a unit in the last place of scale and
+    // smaller than 2^10 of them.  f / scale = h + e / scale, and only the side of h on which its f32 rounding falls
+    // matters: |e / scale| against half a unit of h, two numbers that differ by 2^-23 of them at least (integers over
+    // 2^17 parts of the 24-bit scale; equality would make the quotient a tie between two f32 numbers, which a
+    // quotient of f32 numbers never is), while e * inv is off by 2^-24.  So RN(h + e * inv) falls on the right side.
+    // Rounding to an integer, ties to even, is the addition of 1.5 x 2^23; its low byte is the level.
+    template <typename T>
+    __device__ __forceinline__ uint2 chunk(const uint4& raw) const {
+        constexpr int V = 16 / (int)sizeof(T);
+        constexpr float MAGIC = 12582912.0f;
+        float v[V], far = 0.0f;
+        uint32_t b[V];
+        unpack16<T>(raw, v);
+        const uint64_t inv2 = pack_f32x2(inv, inv), up = pack_f32x2(MAGIC, MAGIC), down = pack_f32x2(-MAGIC, -MAGIC), neg = pack_f32x2(-1.0f, -1.0f);
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {  // two at a time: t, t + magic, (t + magic) - magic, t minus that
+            const uint64_t t = mul_f32x2(pack_f32x2(v[e], v[e + 1]), inv2), u = add_f32x2(t, up);
+            float u0, u1, d0, d1;
+            unpack_f32x2(u, u0, u1);
+            unpack_f32x2(fma_f32x2(add_f32x2(u, down), neg, t), d0, d1);
+            b[e] = __float_as_uint(u0);
+            b[e + 1] = __float_as_uint(u1);
+            far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
         }
+        if (far > 0.49997f) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float t = v[e] * inv, n = __uint_as_float(b[e]) - MAGIC, d = t - n;
+                if (fabsf(d) > 0.49997f) {
+                    const float h = n + copysignf(0.5f, d);
+                    b[e] = __float_as_uint(fmaf(fmaf(-h, scale, v[e]), inv, h) + MAGIC);
+                }
+            }
+        }
+        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < V; e += 4)
+            w[e / 4] = __byte_perm(__byte_perm(b[e], b[e + 1], 0x0040), __byte_perm(b[e + 2], b[e + 3], 0x0040), 0x5410);
+        uint2 r = make_uint2(w[0], w[1]);
+        if (slow || zero) r = exact_chunk<T>(raw, scale, zero);
+        return r;
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(int8_t* dst, const uint4& raw) const {  // dst aligned to the chunk's levels
+        const uint2 r = chunk<T>(raw);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = r;
+        else *reinterpret_cast<uint32_t*>(dst) = r.x;
     }
 };
 // The product of the scales is taken first in every kernel, so that all of them round alike.

@@ -113,6 +113,27 @@ def test_quantize_rows(b, cols, dtype):
         assert torch.equal(q.cpu(), wq) and torch.equal(s.cpu(), ws)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_rows_near_ties(dtype):
+    """Values on and beside every half of every maximum's grid: levels k + 1/2 in all roundings, where the quotient's own
+    rounding decides."""
+    from cmf_b200 import ops
+    g = gen(9)
+    tops = (torch.rand(700, 1, generator=g, device="cuda") * 4 + 0.01).to(dtype).float()
+    tops[:8, 0] = torch.tensor([127.0, 254.0, 3.96875, 1.0, 1e-4, 300.0, 0.49609375, 2.0])
+    halves = (torch.arange(127, device="cuda").float() + 0.5)[None] * (tops / 127)
+    x = torch.cat([tops, halves, -halves, halves * (1 + 2e-7), halves * (1 - 2e-7), halves * (1 + 1.3e-7), halves * (1 - 1.3e-7)], 1)
+    x = torch.cat([x, x[:, :1].expand(-1, (-x.shape[1]) % 16)], 1)
+    x = torch.minimum(torch.maximum(x.to(dtype), -tops.to(dtype)), tops.to(dtype))
+    for scale in (1.0, 2.0 ** -20, 2.0 ** 11) if dtype != torch.float16 else (1.0,):
+        y = (x * scale).contiguous()
+        q, s = ops.quantize_rows(y)
+        wq, ws = ref.quantize_rows(y)
+        assert torch.equal(q.cpu(), wq) and torch.equal(s.cpu(), ws)
+        q, s = ops.quantize_rows(y[:20])                    # a block per row instead of a warp
+        assert torch.equal(q.cpu(), wq[:20]) and torch.equal(s.cpu(), ws[:20])
+
+
 def test_quantize_rows_zeros_ties_tiny_and_non_finite():
     from cmf_b200 import ops
     x = torch.zeros(7, 32, device="cuda")
