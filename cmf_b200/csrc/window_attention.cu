@@ -23,7 +23,7 @@ template <int HDP>
 constexpr int any_smem_floats() { return BM * (HDP + 4) + BN * (HDP + 4) + BN * HDP + BM * (BN + 4); }
 
 template <typename T, int HDP>
-__global__ void __launch_bounds__(THREADS) window_any_kernel(WindowAttnParams p) {
+__global__ void __launch_bounds__(THREADS) window_any_kernel(const __grid_constant__ WindowAttnParams p) {
     extern __shared__ float sm[];
     constexpr int LD = HDP + 4;  // 16-byte rows whose banks shift by four
     float* Qs = sm;                // [BM][LD]

@@ -101,7 +101,7 @@ __device__ __forceinline__ float score(float dot, float scale, float softcap) {
 // result is not finite come here, so that an infinity or a NaN among keys or values that the row does not
 // see cannot reach it, and one that it does see gives what the formula gives.
 template <typename T>
-__device__ __noinline__ void redo_row(const WindowAttnParams& p, const SeqTile& st, int kvh, int row) {
+__device__ __noinline__ void redo_row(const WindowAttnParams& p, SeqTile st, int kvh, int row) {
     const int lane = threadIdx.x & 31;
     const int group = p.nh / p.nkv;
     const int64_t qi = st.q0 + row / group;

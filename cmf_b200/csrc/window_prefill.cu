@@ -132,15 +132,15 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowAttnParams& p, int pos
 template <typename T, int HDP, int POLY_OF_8, bool CAP>
 __global__ void __launch_bounds__(threads<HDP>(), 1)
 window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v, WindowAttnParams p, int tile_tokens, int out_vec) {
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowAttnParams p, int tile_tokens, int out_vec) {
     constexpr int NC = HDP / 64;             // chunks of a K or V tile
     constexpr int VK = SLOT / (HDP * 2);     // keys of a V chunk
     constexpr int SLOTS = slots<HDP>();
     constexpr int TILES = q_tiles<HDP>();
-    const int group = p.nh / p.nkv, kvh = blockIdx.y;
+    const int group = p.nh / p.nkv, kvh = blockIdx.x % p.nkv;
     SeqTile st;
-    // the last tiles of a sequence see the most keys: they start first
-    if (!find_tile(p, (int64_t)gridDim.x - 1 - blockIdx.x, TILES * tile_tokens * group, group, st)) return;
+    // the last tiles of a sequence see the most keys: they start first, all heads of a tile together
+    if (!find_tile(p, (gridDim.x - 1 - blockIdx.x) / p.nkv, TILES * tile_tokens * group, group, st)) return;
     const int i0 = st.tile * TILES * tile_tokens;             // first query of the block
     const int shift = st.k_len - st.q_len;
     const int last_i = min(st.q_len, i0 + TILES * tile_tokens) - 1;
@@ -238,20 +238,29 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             const int steps = two ? 2 * n : n;
             auto k_index = [&](int j) { return (uint32_t)((two ? 2 * j : j == 0 ? 0 : 2 * j - 1) * NC); };
             auto v_index = [&](int j) { return (uint32_t)((two ? 2 * j + 1 : j < n - 1 ? 2 * j + 2 : 2 * n - 1) * NC); };
+            // The thread that issues runs alone, an instruction every few clocks, and a product of 128 x 128 x 16 takes 64:
+            // descriptors are made once and stepped by adding to their address field (16-byte units, 14 bits).
+            const uint64_t q_desc = smem_desc_kmajor(smem_u32(smem), 128), k_desc = smem_desc_kmajor(smem_u32(ring), 128),
+                           v_desc = smem_desc_mn(smem_u32(ring), VK * 128);
+            const bool whole = ksteps == HDP / 16;
+            auto landed = [&](uint32_t idx, uint32_t s) {
+                return __all_sync(0xffffffffu, mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 2)) != 0;
+            };
             auto issue_s = [&](int u) {
                 const int j = two ? u >> 1 : u, x = u & 1;
-                const uint32_t qa = smem_u32(smem + (two ? x : 0) * q_bytes<HDP>());
-                const bool last_use = !two || x == 1;
+                const bool last_use = !two || x == 1, first_use = !two || x == 0;
+                const uint64_t qd = q_desc + (two ? x : 0) * (q_bytes<HDP>() >> 4);
+                const uint32_t d = tmem + x * 128;
+#pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const uint32_t idx = k_index(j) + c, s = idx % SLOTS;
-                    if (!__all_sync(0xffffffffu, mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 2))) return false;
+                    if (first_use && !landed(idx, s)) return false;  // the second query tile comes behind the first
                     tc_fence_after();
                     if (leader) {
-                        const uint32_t ka = smem_u32(ring + s * SLOT);
-                        const int ks = min(4, ksteps - 4 * c);
-                        for (int k = 0; k < ks; ++k)
-                            mma_ss(tmem + x * 128, smem_desc_kmajor(qa + c * QT * 128 + k * 32, 128), smem_desc_kmajor(ka + k * 32, 128), idesc_s,
-                                   (c | k) != 0);
+                        const uint64_t kd = k_desc + s * (SLOT >> 4);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (whole || 4 * c + k < ksteps) mma_ss(d, qd + c * (QT * 128 >> 4) + k * 2, kd + k * 2, idesc_s, (c | k) != 0);
                         if (last_use) tc_commit(&bars->empty[s]);
                     }
                 }
@@ -263,26 +272,31 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 const int j = two ? u >> 1 : u, x = u & 1;
                 const bool last_use = !two || x == 1, first_use = !two || x == 0;
                 // keys of this tile that some row of the block sees; rows of V behind them are zeroed
-                const int live = shift + last_i + 1 - kt.at(j) * KT;
+                const int seen = shift + last_i + 1 - kt.at(j) * KT;
+                const uint32_t d = tmem + o_col + (two ? x * 128 : 0), a = tmem + x * 128;
+#pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const uint32_t idx = v_index(j) + c, s = idx % SLOTS;
-                    if (!__all_sync(0xffffffffu, mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 3))) return false;
-                    if (first_use && live < (c + 1) * VK) {
-                        const int r0 = max(0, live - c * VK);
-                        const int units = (VK - r0) * 8;  // 16-byte pieces of a group of 64 dims
-                        for (int d = 0; d < NC; ++d)
-                            for (int i = lane; i < units; i += 32)
-                                *reinterpret_cast<uint4*>(ring + s * SLOT + d * VK * 128 + r0 * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        fence_proxy_async_smem();
-                        __syncwarp();
+                    if (first_use) {
+                        if (!landed(idx, s)) return false;
+                        if (seen < (c + 1) * VK) {
+                            const int r0 = max(0, seen - c * VK);
+                            const int units = (VK - r0) * 8;  // 16-byte pieces of a group of 64 dims
+                            for (int g = 0; g < NC; ++g)
+                                for (int i = lane; i < units; i += 32)
+                                    *reinterpret_cast<uint4*>(ring + s * SLOT + g * VK * 128 + r0 * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
                     }
                     tc_fence_after();
                     if (leader) {
-                        const uint32_t va = smem_u32(ring + s * SLOT);
+                        const uint64_t vd = v_desc + s * (SLOT >> 4);
 #pragma unroll
-                        for (int k = 0; k < VK / 16; ++k)
-                            mma_ts(tmem + o_col + (two ? x * 128 : 0), tmem + x * 128 + (c * VK + k * 16) / 2, smem_desc_mn(va + k * 2048, VK * 128), idesc_o,
-                                   !(j == 0 && c == 0 && k == 0));
+                        for (int k = 0; k < VK / 16; ++k) {
+                            if (c == 0 && k == 0) mma_ts(d, a, vd, idesc_o, j != 0);
+                            else mma_ts(d, a + (c * VK + k * 16) / 2, vd + k * (2048 >> 4), idesc_o, 1u);
+                        }
                         if (last_use) tc_commit(&bars->empty[s]);
                     }
                 }
@@ -477,7 +491,7 @@ int launch_form(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensor
     }
     const int out_vec = !(reinterpret_cast<uintptr_t>(p.out.p) & 15) && p.out.row % 8 == 0 && p.out.head % 8 == 0 && p.hd % 8 == 0;
     const int64_t blocks = p.q_rows / (q_tiles<HDP>() * tile_tokens) + p.seqs;
-    kernel<<<dim3((unsigned)blocks, p.nkv), threads<HDP>(), smem_bytes<HDP>(), s>>>(tm_q, tm_k, tm_v, p, tile_tokens, out_vec);
+    kernel<<<(unsigned)(blocks * p.nkv), threads<HDP>(), smem_bytes<HDP>(), s>>>(tm_q, tm_k, tm_v, p, tile_tokens, out_vec);
     CMFC_CUDA(cudaGetLastError());
     return OK;
 }
@@ -504,7 +518,9 @@ bool window_prefill_supported(const WindowAttnParams& p, int elem) {
         return !(reinterpret_cast<uintptr_t>(v.p) & 15) && v.row > 0 && v.row < MOST && v.row % 8 == 0 &&
                (heads == 1 || (v.head > 0 && v.head < MOST && v.head % 8 == 0));
     };
-    return elem != ET_F32 && p.scale > 0.0f && p.k_rows > 0 && p.nh / p.nkv <= QT && fits(p.q, p.nh) && fits(p.k, p.nkv) && fits(p.v, p.nkv);
+    const int64_t group = p.nh / p.nkv;
+    return elem != ET_F32 && p.scale > 0.0f && p.k_rows > 0 && group <= QT && (p.q_rows / (QT / group) + p.seqs) * p.nkv < ((int64_t)1 << 31) &&
+           fits(p.q, p.nh) && fits(p.k, p.nkv) && fits(p.v, p.nkv);
 }
 
 int launch_window_prefill(const WindowAttnParams& p, int elem, cudaStream_t s) {

@@ -83,7 +83,7 @@ __device__ __forceinline__ uint32_t tile_at(uint32_t base, int row, int unit) {
 
 template <typename T, int HDP, bool CAP, int W>
 __global__ void __launch_bounds__(32 * (1 + W), (Smem<HDP, W>::PER_SM))
-window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, WindowAttnParams p, int splits) {
+window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowAttnParams p, int splits) {
     using L = Smem<HDP, W>;
     constexpr int NC = HDP / 64, KEYS = L::KEYS, WARPS = L::WARPS, THREADS = L::THREADS;
     // key heads next to each other: their keys lie next to each other too, and DRAM pages are read while open
