@@ -34,9 +34,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 template <int HDP> __host__ __device__ constexpr int q_tiles() { return HDP <= 128 ? 2 : 1; }
 template <int HDP> __host__ __device__ constexpr int slots() { return HDP == 64 ? 12 : 10; }
-template <int HDP> __host__ __device__ constexpr int threads() { return 32 * (2 + 4 * q_tiles<HDP>()); }
+constexpr int THREADS = 32 * (2 + 8);
 template <int HDP> __host__ __device__ constexpr int q_bytes() { return QT * HDP * 2; }
-template <int HDP> __host__ __device__ constexpr int smem_bytes() { return q_tiles<HDP>() * q_bytes<HDP>() + slots<HDP>() * SLOT + 1024 + 512; }
+constexpr int BARS_BYTES = 3072;
+template <int HDP> __host__ __device__ constexpr int smem_bytes() { return q_tiles<HDP>() * q_bytes<HDP>() + slots<HDP>() * SLOT + BARS_BYTES; }
 
 struct Bars {
     uint64_t q_full;
@@ -44,8 +45,15 @@ struct Bars {
     // one of each per stream (query tile, or S buffer); the phase before the one that anybody waits for is
     // always known to be complete, so its parity is enough
     uint64_t s_full[2], p_full[2], o_done[2];
+    // one query tile: reference of the rows' exponentials, handed from warp to warp between the groups; their parts of
+    // the row sums with the reference each is relative to; rows to compute again
+    uint64_t ref_full[2][4];
+    float ref[QT];
+    float2 part[2][QT];
+    uint8_t bad[QT];
     uint32_t tmem_base, abort_flag;
 };
+static_assert(sizeof(Bars) <= BARS_BYTES && smem_bytes<64>() <= 232448 && smem_bytes<128>() <= 232448 && smem_bytes<256>() <= 232448, "barriers and row statistics fit their place");
 
 // kind::f16, f32 accumulator, A and B of one 16-bit type (f16: 0, bf16: 1); b_mn: B is MN-major
 template <typename T>
@@ -85,17 +93,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // quarters of the cap): tanh(y) = y P(y^2) on the FMA pipe, P of degree 5 fitted to tanh(sqrt z) / sqrt z on [0, 0.5625]
 // at Chebyshev points (relative error 3e-8, 1.1e-7 with f32 roundings); else 1 - 2 / (2^(2 y log2 e) + 1) on the special-function unit, which the
 // exponentials of the softmax already fill.
+__device__ __forceinline__ float cap_tanh(float y) { return 1.0f - __fdividef(2.0f, ex2_approx(y * (2.0f * LOG2E)) + 1.0f); }
 __device__ __forceinline__ void softcap_chunk(uint32_t (&v)[32], float to_y, float cap2) {
     uint64_t y2[16];
-    float top = 0.0f;
+    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         y2[i] = mul_f32x2(pack_f32x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), pack_f32x2(to_y, to_y));
         float a, b;
         unpack_f32x2(y2[i], a, b);
-        top = max3_nan(top, fabsf(a), fabsf(b));
+        top[i & 3] = max3_nan(top[i & 3], fabsf(a), fabsf(b));
     }
-    if (__all_sync(0xffffffffu, top <= 0.75f)) {
+    if (__all_sync(0xffffffffu, max_nan(max3_nan(top[0], top[1], top[2]), top[3]) <= 0.75f)) {
         const float c[6] = {1.0f, -0.3333296776f, 0.1332551539f, -0.05334981903f, 0.01959378645f, -0.004723952152f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -113,10 +122,8 @@ __device__ __forceinline__ void softcap_chunk(uint32_t (&v)[32], float to_y, flo
         for (int i = 0; i < 16; ++i) {
             float a, b;
             unpack_f32x2(y2[i], a, b);
-            a = 1.0f - __fdividef(2.0f, ex2_approx(a * (2.0f * LOG2E)) + 1.0f);
-            b = 1.0f - __fdividef(2.0f, ex2_approx(b * (2.0f * LOG2E)) + 1.0f);
-            v[2 * i] = __float_as_uint(a * cap2);
-            v[2 * i + 1] = __float_as_uint(b * cap2);
+            v[2 * i] = __float_as_uint(cap_tanh(a) * cap2);
+            v[2 * i + 1] = __float_as_uint(cap_tanh(b) * cap2);
         }
     }
 }
@@ -130,7 +137,7 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowAttnParams& p, int pos
 }
 
 template <typename T, int HDP, int POLY_OF_8, bool CAP>
-__global__ void __launch_bounds__(threads<HDP>(), 1)
+__global__ void __launch_bounds__(THREADS, 1)
 window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowAttnParams p, int tile_tokens, int out_vec) {
     constexpr int NC = HDP / 64;             // chunks of a K or V tile
@@ -148,8 +155,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const KeyTiles kt = key_tiles(p, st, i0, last_i, KT);
     const int n = kt.count;
 
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];  // whole swizzle patterns of 1024 bytes
     uint8_t* ring = smem + TILES * q_bytes<HDP>();
     Bars* bars = reinterpret_cast<Bars*>(ring + SLOTS * SLOT);
     volatile uint32_t* abort_flag = &bars->abort_flag;
@@ -164,6 +170,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             mbar_init(&bars->s_full[x], 1);
             mbar_init(&bars->p_full[x], 4);
             mbar_init(&bars->o_done[x], 1);
+            for (int w = 0; w < 4; ++w) mbar_init(&bars->ref_full[x][w], 1);
         }
         bars->abort_flag = 0;
         mbar_fence_init();
@@ -177,8 +184,9 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     }
     // rows of a tile that the group does not fill (128 = 42 x 3 + 2) hold zeros: their scores need no mask
     const int used = tile_tokens * group;
-    for (int i = threadIdx.x; i < (QT - used) * 8 * NC * TILES; i += threads<HDP>())
+    for (int i = threadIdx.x; i < (QT - used) * 8 * NC * TILES; i += THREADS)
         *reinterpret_cast<uint4*>(smem + (i / ((QT - used) * 8)) * (QT * 128) + used * 128 + (i % ((QT - used) * 8)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = threadIdx.x; i < QT; i += THREADS) bars->bad[i] = 0;
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
@@ -243,21 +251,27 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             const uint64_t q_desc = smem_desc_kmajor(smem_u32(smem), 128), k_desc = smem_desc_kmajor(smem_u32(ring), 128),
                            v_desc = smem_desc_mn(smem_u32(ring), VK * 128);
             const bool whole = ksteps == HDP / 16;
-            auto landed = [&](uint32_t idx, uint32_t s) {
-                return __all_sync(0xffffffffu, mbar_wait(&bars->full[s], (idx / SLOTS) & 1u, abort_flag, 2)) != 0;
+            // The warp stays together, waits included (descriptors live in uniform registers, which lanes that run
+            // apart would share); only the products and commits are the leader's.
+            auto arrived = [&](uint64_t* bar, uint32_t parity, uint32_t site) {
+                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, site)) != 0;
+            };
+            auto landed = [&](uint32_t index) {
+#pragma unroll
+                for (uint32_t i = 0; i < NC; ++i)
+                    if (!arrived(&bars->full[(index + i) % SLOTS], ((index + i) / SLOTS) & 1u, 2)) return false;
+                return true;
             };
             auto issue_s = [&](int u) {
                 const int j = two ? u >> 1 : u, x = u & 1;
-                const bool last_use = !two || x == 1, first_use = !two || x == 0;
+                const bool last_use = !two || x == 1;  // the second query tile comes behind the first
                 const uint64_t qd = q_desc + (two ? x : 0) * (q_bytes<HDP>() >> 4);
-                const uint32_t d = tmem + x * 128;
+                const uint32_t d = tmem + x * 128, index = k_index(j);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
-                    const uint32_t idx = k_index(j) + c, s = idx % SLOTS;
-                    if (first_use && !landed(idx, s)) return false;  // the second query tile comes behind the first
-                    tc_fence_after();
+                    const uint32_t s = (index + c) % SLOTS;
+                    const uint64_t kd = k_desc + s * (SLOT >> 4);
                     if (leader) {
-                        const uint64_t kd = k_desc + s * (SLOT >> 4);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             if (whole || 4 * c + k < ksteps) mma_ss(d, qd + c * (QT * 128 >> 4) + k * 2, kd + k * 2, idesc_s, (c | k) != 0);
@@ -266,32 +280,16 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 }
                 if (leader) tc_commit(&bars->s_full[x]);
                 __syncwarp();
-                return true;
             };
             auto issue_o = [&](int u) {
                 const int j = two ? u >> 1 : u, x = u & 1;
-                const bool last_use = !two || x == 1, first_use = !two || x == 0;
-                // keys of this tile that some row of the block sees; rows of V behind them are zeroed
-                const int seen = shift + last_i + 1 - kt.at(j) * KT;
-                const uint32_t d = tmem + o_col + (two ? x * 128 : 0), a = tmem + x * 128;
+                const bool last_use = !two || x == 1;
+                const uint32_t d = tmem + o_col + (two ? x * 128 : 0), a = tmem + x * 128, index = v_index(j);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
-                    const uint32_t idx = v_index(j) + c, s = idx % SLOTS;
-                    if (first_use) {
-                        if (!landed(idx, s)) return false;
-                        if (seen < (c + 1) * VK) {
-                            const int r0 = max(0, seen - c * VK);
-                            const int units = (VK - r0) * 8;  // 16-byte pieces of a group of 64 dims
-                            for (int g = 0; g < NC; ++g)
-                                for (int i = lane; i < units; i += 32)
-                                    *reinterpret_cast<uint4*>(ring + s * SLOT + g * VK * 128 + r0 * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                    }
-                    tc_fence_after();
+                    const uint32_t s = (index + c) % SLOTS;
+                    const uint64_t vd = v_desc + s * (SLOT >> 4);
                     if (leader) {
-                        const uint64_t vd = v_desc + s * (SLOT >> 4);
 #pragma unroll
                         for (int k = 0; k < VK / 16; ++k) {
                             if (c == 0 && k == 0) mma_ts(d, a, vd, idesc_o, j != 0);
@@ -302,170 +300,220 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 }
                 if (leader) tc_commit(&bars->o_done[x]);
                 __syncwarp();
-                return true;
             };
-            bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0, abort_flag, 4)) != 0;
-            if (ok) ok = issue_s(0);
-            if (ok && steps > 1) ok = issue_s(1);
+            bool ok = arrived(&bars->q_full, 0, 4) && landed(k_index(0));
+            tc_fence_after();
+            if (ok) issue_s(0);
+            if (ok && steps > 1) {
+                ok = two || landed(k_index(1));
+                if (ok) issue_s(1);
+            }
             for (int u = 0; ok && u < steps; ++u) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[u & 1], (u >> 1) & 1u, abort_flag, 5)) != 0;
+                const int j = two ? u >> 1 : u;
+                // what this step needs from memory, while the softmax is still at work on its P
+                if (!two || (u & 1) == 0) {
+                    ok = landed(v_index(j)) && (u + 2 >= steps || landed(k_index(two ? j + 1 : j + 2)));
+                    if (!ok) break;
+                    const int seen = shift + last_i + 1 - kt.at(j) * KT;  // keys of this tile that some row of the block sees
+                    if (seen < KT) {
+                        for (int c = 0; c < NC; ++c) {
+                            uint8_t* slot = ring + (v_index(j) + c) % SLOTS * SLOT;
+                            const int r0 = max(0, min(VK, seen - c * VK)), units = (VK - r0) * 8;  // 16-byte pieces of a group of 64 dims
+                            for (int g = 0; g < NC; ++g)
+                                for (int i = lane; i < units; i += 32) *reinterpret_cast<uint4*>(slot + g * VK * 128 + r0 * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                ok = arrived(&bars->p_full[u & 1], (u >> 1) & 1u, 5);
                 if (!ok) break;
                 tc_fence_after();
-                ok = issue_o(u);
-                if (ok && u + 2 < steps) ok = issue_s(u + 2);
+                issue_o(u);
+                if (u + 2 < steps) issue_s(u + 2);
             }
         }
     } else {
-        // ---------------- softmax warps: group x of four warps owns query tile x ----------------
-        const int x0 = (warp - 2) >> 2;
+        // ---------------- softmax warps: group x of four warps owns stream x ----------------
+        // Two query tiles: every key tile of query tile x.  One query tile: every other key tile; the reference of
+        // the exponentials, which both groups' P must share, goes from one to the other through shared memory as soon as a
+        // group knows the maximum of its tile, so that one group's exponentials run beside the other's maximum.
+        const int x = (warp - 2) >> 2;
         const int quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-        const int qi = i0 + x0 * tile_tokens + r / group;  // query of this row
+        const int qi = i0 + (two ? x * tile_tokens : 0) + r / group;  // query of this row
         const bool live = r < used && qi < st.q_len;
         const int pos = live ? shift + qi : -1;
-        if (two || x0 == 0) {
-            const float c = p.scale * LOG2E, cap2 = p.softcap * LOG2E, to_y = CAP ? p.scale / p.softcap : 0.0f;
-            float m_ref = -INFINITY, l = 0.0f;
-            bool bad = false, ok = true;
-            for (int j = 0; j < n; ++j) {
-                const int x = two ? x0 : (j & 1);
-                const uint32_t ph = (two ? j : j >> 1) & 1u;
-                // the lanes leave a polling loop one by one: tcgen05.ld wants the warp together
-                if (!__all_sync(0xffffffffu, mbar_wait<20>(&bars->s_full[x], ph, abort_flag, 6))) { ok = false; break; }
-                tc_fence_after();
-                uint32_t v[4][32];
+        const uint32_t s_at = tmem + lane_addr + x * 128, o_at = tmem + lane_addr + o_col + (two ? x * 128 : 0);
+        const float c = p.scale * LOG2E, cap2 = p.softcap * LOG2E, to_y = CAP ? p.scale / p.softcap : 0.0f;
+        const int step = two ? 1 : 2;
+        float m_ref = -INFINITY;                  // reference of O: exponents are s - m_ref
+        float l = 0.0f, l_ref = -INFINITY;        // this thread's part of the row sum and its reference
+        bool bad = false, ok = true;
+        for (int j = two ? 0 : x; j < n; j += step) {
+            const uint32_t ph = (uint32_t)(two ? j : j >> 1) & 1u;
+            // the lanes leave a polling loop one by one: tcgen05.ld wants the warp together
+            if (!__all_sync(0xffffffffu, mbar_wait<20>(&bars->s_full[x], ph, abort_flag, 6))) { ok = false; break; }
+            tc_fence_after();
+            uint32_t v[4][32];
 #pragma unroll
-                for (int ch = 0; ch < 4; ++ch) tmem_ld_x32(tmem + lane_addr + x * 128 + ch * 32, v[ch]);
-                tc_wait_ld();
-                const int j0 = kt.at(j) * KT;
-                const bool whole = r >= used || (j0 + KT - 1 <= pos && ((int64_t)pos - j0 < p.window || j0 + KT <= p.sinks));
-                const bool masked = __any_sync(0xffffffffu, !whole);
-                if (CAP) {
+            for (int ch = 0; ch < 4; ++ch) tmem_ld_x32(s_at + ch * 32, v[ch]);
+            tc_wait_ld();
+            const int j0 = kt.at(j) * KT;
+            const bool whole = r >= used || (j0 + KT - 1 <= pos && ((int64_t)pos - j0 < p.window || j0 + KT <= p.sinks));
+            const bool masked = __any_sync(0xffffffffu, !whole);
+            if (masked) {
 #pragma unroll
-                    for (int ch = 0; ch < 4; ++ch) {
-                        if (masked) {  // what is not seen must not choose the path
-                            const uint32_t bits = seen_bits(p, pos, j0 + ch * 32);
+                for (int ch = 0; ch < 4; ++ch) {
+                    const uint32_t bits = r >= used ? 0xffffffffu : seen_bits(p, pos, j0 + ch * 32);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (!(bits >> i & 1u)) v[ch][i] = 0u;
-                        }
-                        softcap_chunk(v[ch], to_y, cap2);
-                    }
+                    for (int i = 0; i < 32; ++i)
+                        if (!(bits >> i & 1u)) v[ch][i] = 0xff800000u;
                 }
-                if (masked) {
+            }
+            float mxs[8];
 #pragma unroll
-                    for (int ch = 0; ch < 4; ++ch) {
-                        const uint32_t bits = seen_bits(p, pos, j0 + ch * 32);
+            for (int a = 0; a < 8; ++a) mxs[a] = -INFINITY;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+                for (int i = 0; i < 32; i += 2)
+                    mxs[(i >> 1) & 7] = max3_nan(mxs[(i >> 1) & 7], __uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1]));
+            const float mx = max_nan(max3_nan(max3_nan(mxs[0], mxs[1], mxs[2]), mxs[3], mxs[4]), max3_nan(mxs[5], mxs[6], mxs[7]));
+            // the cap keeps the order: the largest capped score is the capped largest score
+            const float m_cand = !CAP ? mx * c : mx == -INFINITY ? mx : cap2 * cap_tanh(mx * to_y);
+            bad = bad || m_cand != m_cand;
+            if (!two && j > 0) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&bars->ref_full[x ^ 1][quarter], (uint32_t)((j - 1) >> 1) & 1u, abort_flag, 9))) { ok = false; break; }
+                m_ref = bars->ref[r];
+            }
+            const bool moved = m_cand > m_ref + 8.0f || (m_ref == -INFINITY && m_cand > -INFINITY);
+            const float alpha = moved ? ex2_approx(m_ref - m_cand) : 1.0f;
+            if (moved) m_ref = m_cand;
+            if (!two) {
+                bars->ref[r] = m_ref;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->ref_full[x][quarter]);
+            }
+            if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                // P V of the query tile's previous key tile has to be in O (with two query tiles S(j) was issued
+                // behind it, with two S buffers before it); the next one waits for this warp's P
+                if (!__all_sync(0xffffffffu, mbar_wait(&bars->o_done[two ? x : x ^ 1], (uint32_t)(two ? j - 1 : (j - 1) >> 1) & 1u, abort_flag, 7))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll 1
+                for (int ch = 0; ch < (p.hd + 7) / 8; ++ch) {
+                    uint32_t o[8];
+                    tmem_ld_x8(o_at + ch * 8, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    tmem_st_x8(o_at + ch * 8, o);
+                }
+            }
+            if (l_ref != m_ref) {
+                l *= ex2_approx(l_ref - m_ref);
+                l_ref = m_ref;
+            }
+            const float ref = m_ref == -INFINITY ? 0.0f : m_ref;
+            const uint64_t c2 = pack_f32x2(c, c), nm2 = pack_f32x2(-ref, -ref);
+            uint64_t sums[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+                if (CAP) {
+                    softcap_chunk(v[ch], to_y, cap2);
+                    if (masked) {
+                        const uint32_t bits = r >= used ? 0xffffffffu : seen_bits(p, pos, j0 + ch * 32);
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (!(bits >> i & 1u)) v[ch][i] = 0xff800000u;
                     }
                 }
-                float mxs[8];
+                uint32_t pk[16];
 #pragma unroll
-                for (int a = 0; a < 8; ++a) mxs[a] = -INFINITY;
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        mxs[(i >> 1) & 7] = max3_nan(mxs[(i >> 1) & 7], __uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1]));
-                const float mx = max_nan(max3_nan(max3_nan(mxs[0], mxs[1], mxs[2]), mxs[3], mxs[4]), max3_nan(mxs[5], mxs[6], mxs[7]));
-                const float m_cand = CAP ? mx : mx * c;
-                bad = bad || m_cand != m_cand;
-                const bool moved = m_cand > m_ref + 8.0f || (m_ref == -INFINITY && m_cand > -INFINITY);
-                if (__any_sync(0xffffffffu, moved)) {
-                    const float alpha = moved ? ex2_approx(m_ref - m_cand) : 1.0f;
-                    if (moved) m_ref = m_cand;
-                    l *= alpha;
-                    if (j > 0) {
-                        // P V of the tile's previous key tile has to be in O (with two query tiles S(j) was issued
-                        // behind it, with two S buffers before it); the next one waits for this warp's P
-                        if (!__all_sync(0xffffffffu, mbar_wait(&bars->o_done[two ? x0 : (j - 1) & 1], (uint32_t)(two ? j - 1 : (j - 1) >> 1) & 1u, abort_flag, 7))) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int ch = 0; ch < (p.hd + 7) / 8; ++ch) {
-                            uint32_t o[8];
-                            const uint32_t at = tmem + lane_addr + o_col + (two ? x0 * 128 : 0) + ch * 8;
-                            tmem_ld_x8(at, o);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st_x8(at, o);
-                        }
+                for (int i = 0; i < 32; i += 2) {
+                    float t0, t1, e0, e1;
+                    const uint64_t sv = pack_f32x2(__uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1]));
+                    unpack_f32x2(CAP ? add_f32x2(sv, nm2) : fma_f32x2(sv, c2, nm2), t0, t1);
+                    if ((((i >> 1) & 7) * POLY_OF_8) % 8 < POLY_OF_8) {
+                        ex2_poly_x2<true>(t0, t1, e0, e1);
+                    } else {
+                        e0 = ex2_approx(t0);
+                        e1 = ex2_approx(t1);
                     }
+                    sums[(i >> 1) & 3] = add_f32x2(sums[(i >> 1) & 3], pack_f32x2(e0, e1));
+                    pk[i >> 1] = pack2<T>(e0, e1);
                 }
-                const float ref = m_ref == -INFINITY ? 0.0f : m_ref;
-                const uint64_t c2 = pack_f32x2(c, c), nm2 = pack_f32x2(-ref, -ref);
-                uint64_t sums[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float t0, t1, e0, e1;
-                        const uint64_t sv = pack_f32x2(__uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1]));
-                        unpack_f32x2(CAP ? add_f32x2(sv, nm2) : fma_f32x2(sv, c2, nm2), t0, t1);
-                        if ((((i >> 1) & 7) * POLY_OF_8) % 8 < POLY_OF_8) {
-                            ex2_poly_x2<true>(t0, t1, e0, e1);
-                        } else {
-                            e0 = ex2_approx(t0);
-                            e1 = ex2_approx(t1);
-                        }
-                        sums[(i >> 1) & 3] = add_f32x2(sums[(i >> 1) & 3], pack_f32x2(e0, e1));
-                        pk[i >> 1] = pack2<T>(e0, e1);
-                    }
-                    tmem_st_x16(tmem + lane_addr + x * 128 + ch * 16, pk);
-                }
-                tc_wait_st();
-                {
-                    float s0, s1;
-                    unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), s0, s1);
-                    l += s0 + s1;
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->p_full[x]);
+                tmem_st_x16(s_at + ch * 16, pk);
             }
-            if (n > 0 && ok)
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[two ? x0 : (n - 1) & 1], (uint32_t)(two ? n - 1 : (n - 1) >> 1) & 1u, abort_flag, 8)) != 0;
-            if (ok) {
-                tc_fence_after();
-                const float inv = pos >= 0 ? 1.0f / l : 0.0f;
-                T* dst = static_cast<T*>(const_cast<void*>(p.out.p)) + (st.q0 + qi) * p.out.row + (int64_t)(kvh * group + r % group) * p.out.head;
-                for (int ch = 0; ch < (p.hd + 15) / 16; ++ch) {
-                    uint32_t o[16];
-                    __syncwarp();  // the stores below leave lanes apart, tcgen05.ld wants the warp together
-                    if (n > 0) {
-                        tmem_ld_x16(tmem + lane_addr + o_col + (two ? x0 * 128 : 0) + ch * 16, o);
-                        tc_wait_ld();
-                    }
-                    float f[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        f[i] = pos >= 0 && n > 0 ? __uint_as_float(o[i]) * inv : 0.0f;  // a query that sees no key: zeros
-                        bad = bad || !isfinite(f[i]);
-                    }
-                    if (live) {
-                        if (out_vec) {
-                            *reinterpret_cast<uint4*>(dst + ch * 16) = pack16<T>(f);
-                            if (ch * 16 + 8 < p.hd) *reinterpret_cast<uint4*>(dst + ch * 16 + 8) = pack16<T>(f + 8);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (ch * 16 + i < p.hd) dst[ch * 16 + i] = from_f32<T>(f[i]);
-                        }
-                    }
+            tc_wait_st();
+            {
+                float s0, s1;
+                unpack_f32x2(add_f32x2(add_f32x2(sums[0], sums[1]), add_f32x2(sums[2], sums[3])), s0, s1);
+                l += s0 + s1;
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->p_full[x]);
+        }
+        if (!two) {
+            // The groups' parts of the row sum meet; all eight warps get here whether or not a wait gave up.
+            bars->part[x][r] = make_float2(l, l_ref);
+            if (bad) bars->bad[r] = 1;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float2 other = bars->part[x ^ 1][r];
+            const float m = fmaxf(l_ref, other.y);  // the later of the two: a reference only grows
+            l = (l_ref == m ? l : l * ex2_approx(l_ref - m)) + (other.y == m ? other.x : other.x * ex2_approx(other.y - m));
+            bad = bars->bad[r] != 0;
+        }
+        if (n > 0 && ok) {
+            const int last = two ? x : (n - 1) & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[last], (uint32_t)(two ? n - 1 : (n - 1) >> 1) & 1u, abort_flag, 8)) != 0;
+        }
+        if (ok) {
+            tc_fence_after();
+            const float inv = pos >= 0 ? 1.0f / l : 0.0f;
+            T* dst = static_cast<T*>(const_cast<void*>(p.out.p)) + (st.q0 + qi) * p.out.row + (int64_t)(kvh * group + r % group) * p.out.head;
+            // one query tile: each group writes half of the row
+            const int chunks = (p.hd + 15) / 16, half = (chunks + 1) / 2;
+            const int ch0 = two || x == 0 ? 0 : half, ch1 = two || x == 1 ? chunks : half;
+            for (int ch = ch0; ch < ch1; ++ch) {
+                uint32_t o[16];
+                __syncwarp();  // the stores below leave lanes apart, tcgen05.ld wants the warp together
+                if (n > 0) {
+                    tmem_ld_x16(o_at + ch * 16, o);
+                    tc_wait_ld();
                 }
-                unsigned redo = __ballot_sync(0xffffffffu, bad && pos >= 0);
-                __syncwarp();
-                for (; redo; redo &= redo - 1) {
-                    const int row = (i0 + x0 * tile_tokens) * group + quarter * 32 + __ffs(redo) - 1;
-                    redo_row<T>(p, st, kvh, row);
+                float f[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    f[i] = pos >= 0 && n > 0 ? __uint_as_float(o[i]) * inv : 0.0f;  // a query that sees no key: zeros
+                    bad = bad || !isfinite(f[i]);
+                }
+                if (live) {
+                    if (out_vec) {
+                        *reinterpret_cast<uint4*>(dst + ch * 16) = pack16<T>(f);
+                        if (ch * 16 + 8 < p.hd) *reinterpret_cast<uint4*>(dst + ch * 16 + 8) = pack16<T>(f + 8);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (ch * 16 + i < p.hd) dst[ch * 16 + i] = from_f32<T>(f[i]);
+                    }
                 }
             }
+            if (!two) {
+                // either group may have found the row bad; both have written their halves when one computes it again
+                if (bad) bars->bad[r] = 1;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                bad = x == 0 && bars->bad[r] != 0;
+            }
+            unsigned redo = __ballot_sync(0xffffffffu, bad && pos >= 0);
+            __syncwarp();
+            for (; redo; redo &= redo - 1) redo_row<T>(p, st, kvh, (i0 + (two ? x * tile_tokens : 0)) * group + quarter * 32 + __ffs(redo) - 1);
+        } else if (!two) {
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // the other group may wait here
         }
     }
 
@@ -491,7 +539,7 @@ int launch_form(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensor
     }
     const int out_vec = !(reinterpret_cast<uintptr_t>(p.out.p) & 15) && p.out.row % 8 == 0 && p.out.head % 8 == 0 && p.hd % 8 == 0;
     const int64_t blocks = p.q_rows / (q_tiles<HDP>() * tile_tokens) + p.seqs;
-    kernel<<<(unsigned)(blocks * p.nkv), threads<HDP>(), smem_bytes<HDP>(), s>>>(tm_q, tm_k, tm_v, p, tile_tokens, out_vec);
+    kernel<<<(unsigned)(blocks * p.nkv), THREADS, smem_bytes<HDP>(), s>>>(tm_q, tm_k, tm_v, p, tile_tokens, out_vec);
     CMFC_CUDA(cudaGetLastError());
     return OK;
 }
