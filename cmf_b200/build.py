@@ -7,7 +7,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libcmf_cuda.so")
 SOURCES = ["gemm_dequant.cu", "gemm_dequant_pair.cu", "attention.cu", "rowops.cu", "codec_kernels.cu", "runtime.cu", "api.cu", "noalloc.cu", "selftest.cu",
            "conv_f16x2.cu", "vae_kernels.cu", "vae.cu", "gemma_kernels.cu", "gemma.cu",
-           "head_norm_rope.cu", "i8_gemm.cu", "i8_gemm_pair.cu", "window_attention.cu", "window_prefill.cu", "window_tokens.cu", "text_ops.cu"]
+           "head_norm_rope.cu", "i8_gemm.cu", "i8_gemm_pair.cu", "window_attention.cu", "window_prefill.cu", "window_f32.cu", "window_tokens.cu", "text_ops.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--expt-relaxed-constexpr"]
 

@@ -204,6 +204,7 @@ int launch_window_attention(const WindowAttnParams& p, int elem, int num_sms, cu
     // up to 32 rows a sequence on average: the key axis is what there is to split
     if (p.q_rows * (p.nh / p.nkv) <= 32 * (int64_t)p.seqs && window_tokens_supported(p, elem)) return launch_window_tokens(p, elem, num_sms, s);
     if (window_prefill_supported(p, elem)) return launch_window_prefill(p, elem, s);
+    if (window_f32_supported(p, elem)) return launch_window_f32(p, s);
     return launch_window_any(p, elem, s);
 }
 

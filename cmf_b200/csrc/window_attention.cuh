@@ -7,6 +7,8 @@ namespace cmfc {
 int launch_window_any(const WindowAttnParams& p, int elem, cudaStream_t s);
 bool window_prefill_supported(const WindowAttnParams& p, int elem);
 int launch_window_prefill(const WindowAttnParams& p, int elem, cudaStream_t s);
+bool window_f32_supported(const WindowAttnParams& p, int elem);
+int launch_window_f32(const WindowAttnParams& p, cudaStream_t s);
 bool window_tokens_supported(const WindowAttnParams& p, int elem);
 int launch_window_tokens(const WindowAttnParams& p, int elem, int num_sms, cudaStream_t s);
 
