@@ -1,5 +1,7 @@
 // Shared by the windowed-attention kernels: which rows and keys a block works on, the mask and the score.
 #pragma once
+#include <algorithm>
+
 #include "text_ops.cuh"
 
 namespace cmfc {
@@ -15,6 +17,15 @@ int launch_window_tokens(const WindowAttnParams& p, int elem, int num_sms, cudaS
 // Upper bound of the row tiles of all sequences: every sequence adds at most one partial tile.
 inline int64_t max_tiles(const WindowAttnParams& p, int rows_per_tile) {
     return p.q_rows * (p.nh / p.nkv) / rows_per_tile + p.seqs;
+}
+
+// The lengths are on the device: where a launch is cut by how much there is to do, the host goes by the tensors' sizes
+// and the window, and a wrong guess costs time only.
+inline int64_t window_items(const WindowAttnParams& p, int rows_per_tile) {  // row tiles x key heads
+    return std::max<int64_t>(1, (p.q_rows * (p.nh / p.nkv) / p.seqs + rows_per_tile - 1) / rows_per_tile) * p.seqs * p.nkv;
+}
+inline int64_t window_range(const WindowAttnParams& p) {  // keys of a row
+    return std::min<int64_t>((int64_t)p.window + p.sinks, std::max<int64_t>(1, p.k_rows / p.seqs));
 }
 
 #ifdef __CUDACC__

@@ -14,7 +14,6 @@
 // finite are computed again key by key (redo_row).
 #include <cooperative_groups.h>
 
-#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -365,14 +364,6 @@ window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     if (splits > 1) cluster.sync();  // nobody's shared memory goes away while another block reads it
 }
 
-// The lengths are on the device: the host goes by the tensors' sizes and the window, and a wrong guess costs time only.
-int64_t items_of(const WindowAttnParams& p) {
-    return std::max<int64_t>(1, (p.q_rows * (p.nh / p.nkv) / p.seqs + ROWS - 1) / ROWS) * p.seqs * p.nkv;
-}
-int64_t range_of(const WindowAttnParams& p) {
-    return std::min<int64_t>((int64_t)p.window + p.sinks, std::max<int64_t>(1, p.k_rows / p.seqs));
-}
-
 template <typename T, int HDP, bool CAP, int W>
 int launch_form(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, cudaStream_t s) {
     static std::atomic<int> clusters_of[64][MAX_SPLITS + 1];  // clusters that run at once, a property of the device
@@ -401,7 +392,7 @@ int launch_form(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAt
     // Cut the key axis only as far as all shares still run at once and keep 128 keys: a cluster waits until all of its
     // blocks find room (64 sequences x 4 key heads of 256 x 4096 keys: uncut 164 us, in two 192, in four 226; one
     // sequence x 8 heads of 128 x 4096 keys: uncut 40 us, in two 24, in four 16, in eight 12).
-    const int64_t items = items_of(p), range = range_of(p);
+    const int64_t items = window_items(p, ROWS), range = window_range(p);
     int splits = 1;
     while (splits < MAX_SPLITS && items <= clusters_of[dev & 63][2 * splits] && range / (2 * splits) >= 128) splits *= 2;
     attr[0].val.clusterDim.x = splits;
@@ -416,7 +407,7 @@ int launch_hdp(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAtt
     // blocks per SM, one of which starts or ends while the other reads (64 sequences x 8 heads of 128 x 4096 keys: 167 us,
     // with eight warps 188).  Heads of 256 leave room for the tiles of four warps.
     if constexpr (HDP <= 128) {
-        if (items_of(p) <= num_sms / 2)
+        if (window_items(p, ROWS) <= num_sms / 2)
             return p.softcap > 0.0f ? launch_form<T, HDP, true, 8>(tm_k, tm_v, p, s) : launch_form<T, HDP, false, 8>(tm_k, tm_v, p, s);
     }
     return p.softcap > 0.0f ? launch_form<T, HDP, true, 4>(tm_k, tm_v, p, s) : launch_form<T, HDP, false, 4>(tm_k, tm_v, p, s);
