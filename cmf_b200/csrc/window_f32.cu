@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
         copy16(Qs + r * LD + d, live ? qp + (st.q0 + row / group) * p.q.row + (int64_t)(kvh * group + row % group) * p.q.head + d : qp, live);
     }
     if (kt.count) fetch(buf, kp, p.k.row, kt.at(0) * BN);
-    float m[A], l[A], acc[A][HDP / 16];
+    float m[A], l[A];
+    uint64_t acc[A][HDP / 32];  // pairs of dims
     int pos[A];
 #pragma unroll
     for (int a = 0; a < A; ++a) {
@@ -73,7 +74,7 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
         const int row = r0 + ty * A + a;
         pos[a] = row < rows ? st.k_len - st.q_len + row / group : -1;
 #pragma unroll
-        for (int c = 0; c < HDP / 16; ++c) acc[a][c] = 0.0f;
+        for (int c = 0; c < HDP / 32; ++c) acc[a][c] = 0ull;
     }
     float *Ks = buf, *Vs = buf + BN * LD;
     for (int it = 0; it < kt.count; ++it) {
@@ -81,28 +82,36 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
         fetch(Vs, vp, p.v.row, j0);
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // K(it), and Q
         __syncthreads();
-        float s[A][4];
+        // even and odd dims in the two halves of a packed sum: one instruction for two FMA
+        uint64_t s2[A][4];
 #pragma unroll
         for (int a = 0; a < A; ++a)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) s[a][b] = 0.0f;
+            for (int b = 0; b < 4; ++b) s2[a][b] = 0ull;
 #pragma unroll 4
         for (int d = 0; d < HDP; d += 4) {
-            float4 qv[A], kv[4];
+            ulonglong2 qv[A], kv[4];
 #pragma unroll
-            for (int a = 0; a < A; ++a) qv[a] = *reinterpret_cast<const float4*>(Qs + (ty * A + a) * LD + d);
+            for (int a = 0; a < A; ++a) qv[a] = *reinterpret_cast<const ulonglong2*>(Qs + (ty * A + a) * LD + d);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) kv[b] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * b) * LD + d);
+            for (int b = 0; b < 4; ++b) kv[b] = *reinterpret_cast<const ulonglong2*>(Ks + (tx + 16 * b) * LD + d);
 #pragma unroll
             for (int a = 0; a < A; ++a)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    s[a][b] = fmaf(qv[a].x, kv[b].x, s[a][b]);
-                    s[a][b] = fmaf(qv[a].y, kv[b].y, s[a][b]);
-                    s[a][b] = fmaf(qv[a].z, kv[b].z, s[a][b]);
-                    s[a][b] = fmaf(qv[a].w, kv[b].w, s[a][b]);
+                    s2[a][b] = fma_f32x2(qv[a].x, kv[b].x, s2[a][b]);
+                    s2[a][b] = fma_f32x2(qv[a].y, kv[b].y, s2[a][b]);
                 }
         }
+        float s[A][4];
+#pragma unroll
+        for (int a = 0; a < A; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float lo, hi;
+                unpack_f32x2(s2[a][b], lo, hi);
+                s[a][b] = lo + hi;
+            }
 #pragma unroll
         for (int a = 0; a < A; ++a) {
             float top = -INFINITY;
@@ -127,8 +136,9 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
 #pragma unroll
             for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             l[a] = l[a] * alpha + sum;
+            const uint64_t alpha2 = pack_f32x2(alpha, alpha);
 #pragma unroll
-            for (int c = 0; c < HDP / 16; ++c) acc[a][c] *= alpha;
+            for (int c = 0; c < HDP / 32; ++c) acc[a][c] = mul_f32x2(acc[a][c], alpha2);
         }
         __syncthreads();  // everybody is done with K(it)
         if (it + 1 < kt.count) {
@@ -147,14 +157,13 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
             for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
                 for (int c = 0; c < HDP / 64; ++c) {
-                    const float4 v = *reinterpret_cast<const float4*>(Vs + (j + jj) * LD + c * 64 + tx * 4);
+                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(Vs + (j + jj) * LD + c * 64 + tx * 4);
 #pragma unroll
                     for (int a = 0; a < A; ++a) {
                         const float w = jj == 0 ? pw[a].x : jj == 1 ? pw[a].y : jj == 2 ? pw[a].z : pw[a].w;
-                        acc[a][c * 4] = fmaf(w, v.x, acc[a][c * 4]);
-                        acc[a][c * 4 + 1] = fmaf(w, v.y, acc[a][c * 4 + 1]);
-                        acc[a][c * 4 + 2] = fmaf(w, v.z, acc[a][c * 4 + 2]);
-                        acc[a][c * 4 + 3] = fmaf(w, v.w, acc[a][c * 4 + 3]);
+                        const uint64_t w2 = pack_f32x2(w, w);
+                        acc[a][c * 2] = fma_f32x2(w2, v.x, acc[a][c * 2]);
+                        acc[a][c * 2 + 1] = fma_f32x2(w2, v.y, acc[a][c * 2 + 1]);
                     }
                 }
         }
@@ -169,11 +178,16 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
         bool fine = true;
         float* dst = static_cast<float*>(const_cast<void*>(p.out.p)) + (st.q0 + row / group) * p.out.row + (int64_t)(kvh * group + row % group) * p.out.head;
 #pragma unroll
-        for (int c = 0; c < HDP / 16; ++c) {
-            const int d = (c >> 2) * 64 + tx * 4 + (c & 3);
-            const float o = any ? acc[a][c] * inv : 0.0f;
-            fine = fine && isfinite(o);
-            if (row < rows && d < p.hd) dst[d] = o;
+        for (int c = 0; c < HDP / 32; ++c) {
+            const int d = (c >> 1) * 64 + tx * 4 + (c & 1) * 2;
+            float o[2];
+            unpack_f32x2(acc[a][c], o[0], o[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                o[e] = any ? o[e] * inv : 0.0f;
+                fine = fine && isfinite(o[e]);
+                if (row < rows && d + e < p.hd) dst[d + e] = o[e];
+            }
         }
         const unsigned bad = __ballot_sync(0xffffffffu, row < rows && !fine);
         if (bad & 0xffffu) redo |= 1u << a;   // rows ty * A + a of the two half warps
