@@ -89,44 +89,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// cap * log2(e) * tanh(s * scale / cap) for a chunk of a row.  |y| <= 0.75 in the whole warp (scores up to three
-// quarters of the cap): tanh(y) = y P(y^2) on the FMA pipe, P of degree 5 fitted to tanh(sqrt z) / sqrt z on [0, 0.5625]
-// at Chebyshev points (relative error 3e-8, 1.1e-7 with f32 roundings); else 1 - 2 / (2^(2 y log2 e) + 1) on the special-function unit, which the
-// exponentials of the softmax already fill.
+// Soft cap.  Where all |y| = |score / cap| of a warp's rows are at most 0.75, tanh(y) = y P(y^2) on the FMA pipe, P of degree 5
+// fitted to tanh(sqrt z) / sqrt z on [0, 0.5625] at Chebyshev points (relative error 3e-8, 1.1e-7 with f32 roundings);
+// else 1 - 2 / (2^(2 y log2 e) + 1) on the special-function unit, which the exponentials of the softmax already fill.
 __device__ __forceinline__ float cap_tanh(float y) { return 1.0f - __fdividef(2.0f, ex2_approx(y * (2.0f * LOG2E)) + 1.0f); }
-__device__ __forceinline__ void softcap_chunk(uint32_t (&v)[32], float to_y, float cap2) {
-    uint64_t y2[16];
-    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        y2[i] = mul_f32x2(pack_f32x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), pack_f32x2(to_y, to_y));
-        float a, b;
-        unpack_f32x2(y2[i], a, b);
-        top[i & 3] = max3_nan(top[i & 3], fabsf(a), fabsf(b));
-    }
-    if (__all_sync(0xffffffffu, max_nan(max3_nan(top[0], top[1], top[2]), top[3]) <= 0.75f)) {
-        const float c[6] = {1.0f, -0.3333296776f, 0.1332551539f, -0.05334981903f, 0.01959378645f, -0.004723952152f};
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint64_t z = mul_f32x2(y2[i], y2[i]);
-            uint64_t q = pack_f32x2(c[5], c[5]);
-#pragma unroll
-            for (int k = 4; k >= 0; --k) q = fma_f32x2(q, z, pack_f32x2(c[k], c[k]));
-            float a, b;
-            unpack_f32x2(mul_f32x2(mul_f32x2(y2[i], pack_f32x2(cap2, cap2)), q), a, b);
-            v[2 * i] = __float_as_uint(a);
-            v[2 * i + 1] = __float_as_uint(b);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float a, b;
-            unpack_f32x2(y2[i], a, b);
-            v[2 * i] = __float_as_uint(cap_tanh(a) * cap2);
-            v[2 * i + 1] = __float_as_uint(cap_tanh(b) * cap2);
-        }
-    }
-}
 
 // bit i: the row at position pos sees key j0 + i
 __device__ __forceinline__ uint32_t seen_bits(const WindowAttnParams& p, int pos, int j0) {
@@ -346,6 +312,13 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         const int pos = live ? shift + qi : -1;
         const uint32_t s_at = tmem + lane_addr + x * 128, o_at = tmem + lane_addr + o_col + (two ? x * 128 : 0);
         const float c = p.scale * LOG2E, cap2 = p.softcap * LOG2E, to_y = CAP ? p.scale / p.softcap : 0.0f;
+        // P's coefficients for a score s instead of y = s to_y, times cap log2(e)
+        float cap_c[6] = {1.0f, -0.3333296776f, 0.1332551539f, -0.0533498190f, 0.0195937864f, -0.0047239522f};
+        if (CAP) {
+            float f = cap2 * to_y;
+#pragma unroll
+            for (int k = 0; k < 6; ++k, f *= to_y * to_y) cap_c[k] *= f;
+        }
         const int step = two ? 1 : 2;
         float m_ref = -INFINITY;                  // reference of O: exponents are s - m_ref
         float l = 0.0f, l_ref = -INFINITY;        // this thread's part of the row sum and its reference
@@ -380,6 +353,16 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                 for (int i = 0; i < 32; i += 2)
                     mxs[(i >> 1) & 7] = max3_nan(mxs[(i >> 1) & 7], __uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1]));
             const float mx = max_nan(max3_nan(max3_nan(mxs[0], mxs[1], mxs[2]), mxs[3], mxs[4]), max3_nan(mxs[5], mxs[6], mxs[7]));
+            bool small = false;  // every score of the warp's rows lies where the polynomial holds (a masked tile's do not)
+            if (CAP) {
+                float mns[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+                        mns[(i >> 1) & 3] = fminf(mns[(i >> 1) & 3], fminf(__uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1])));
+                small = __all_sync(0xffffffffu, fmaxf(mx, -fminf(fminf(mns[0], mns[1]), fminf(mns[2], mns[3]))) * to_y <= 0.75f);
+            }
             // the cap keeps the order: the largest capped score is the capped largest score
             const float m_cand = !CAP ? mx * c : mx == -INFINITY ? mx : cap2 * cap_tanh(mx * to_y);
             bad = bad || m_cand != m_cand;
@@ -420,33 +403,46 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             const float ref = m_ref == -INFINITY ? 0.0f : m_ref;
             const uint64_t c2 = pack_f32x2(c, c), nm2 = pack_f32x2(-ref, -ref);
             uint64_t sums[4] = {0ull, 0ull, 0ull, 0ull};
+            // exponents of two scores -> weights, their sum and P; one straight run of code for either form of the cap
+            auto weights = [&](auto exponent) {
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-                if (CAP) {
-                    softcap_chunk(v[ch], to_y, cap2);
-                    if (masked) {
-                        const uint32_t bits = r >= used ? 0xffffffffu : seen_bits(p, pos, j0 + ch * 32);
+                for (int ch = 0; ch < 4; ++ch) {
+                    uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!(bits >> i & 1u)) v[ch][i] = 0xff800000u;
+                    for (int i = 0; i < 32; i += 2) {
+                        float t0, t1, e0, e1;
+                        unpack_f32x2(exponent(pack_f32x2(__uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1]))), t0, t1);
+                        if ((((i >> 1) & 7) * POLY_OF_8) % 8 < POLY_OF_8) {
+                            ex2_poly_x2<true>(t0, t1, e0, e1);
+                        } else {
+                            e0 = ex2_approx(t0);
+                            e1 = ex2_approx(t1);
+                        }
+                        sums[(i >> 1) & 3] = add_f32x2(sums[(i >> 1) & 3], pack_f32x2(e0, e1));
+                        pk[i >> 1] = pack2<T>(e0, e1);
                     }
+                    tmem_st_x16(s_at + ch * 16, pk);
                 }
-                uint32_t pk[16];
+            };
+            if (!CAP) {
+                weights([&](uint64_t sv) { return fma_f32x2(sv, c2, nm2); });
+            } else if (small) {
+                weights([&](uint64_t sv) {  // seven instructions for two scores: s P'(s^2) - ref
+                    const uint64_t z = mul_f32x2(sv, sv);
+                    uint64_t q = pack_f32x2(cap_c[5], cap_c[5]);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    float t0, t1, e0, e1;
-                    const uint64_t sv = pack_f32x2(__uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1]));
-                    unpack_f32x2(CAP ? add_f32x2(sv, nm2) : fma_f32x2(sv, c2, nm2), t0, t1);
-                    if ((((i >> 1) & 7) * POLY_OF_8) % 8 < POLY_OF_8) {
-                        ex2_poly_x2<true>(t0, t1, e0, e1);
-                    } else {
-                        e0 = ex2_approx(t0);
-                        e1 = ex2_approx(t1);
-                    }
-                    sums[(i >> 1) & 3] = add_f32x2(sums[(i >> 1) & 3], pack_f32x2(e0, e1));
-                    pk[i >> 1] = pack2<T>(e0, e1);
+                    for (int k = 4; k >= 0; --k) q = fma_f32x2(q, z, pack_f32x2(cap_c[k], cap_c[k]));
+                    return fma_f32x2(sv, q, nm2);
+                });
+            } else {
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                    const uint32_t bits = r >= used || !masked ? 0xffffffffu : seen_bits(p, pos, j0 + ch * 32);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        v[ch][i] = bits >> i & 1u ? __float_as_uint(cap_tanh(__uint_as_float(v[ch][i]) * to_y) * cap2) : 0xff800000u;
                 }
-                tmem_st_x16(s_at + ch * 16, pk);
+                weights([&](uint64_t sv) { return add_f32x2(sv, nm2); });
             }
             tc_wait_st();
             {
