@@ -10,8 +10,8 @@
 //   warp 1         MMA issuer (even CTA)
 //   warps 2 - 9    epilogue: tcgen05.ld, integer -> f32, both scales, rounded to the output type, 32 x 32 chunks staged
 //                  in shared memory and written by TMA stores (plain stores where the output is not 16-byte aligned)
-// Few tiles (a batch of some hundred tokens, a narrow matrix): the K axis is cut into 2 or 4 slices, one per
-// pair of a cluster of 4 or 8 CTAs; the slices' integer sums meet over distributed shared memory in the
+// Few tiles (a batch of some hundred tokens, a narrow matrix): the K axis is cut into 2 to 4 slices, one per
+// pair of a cluster of 4 to 8 CTAs; the slices' integer sums meet over distributed shared memory in the
 // stages' own space.  Integer sums are exact, so neither the cut nor the batch changes a bit of the result.
 //
 // Bound: the tensor pipe, and close behind it L2 -> SM (a 256 x 256 tile takes 64 KB per 128 levels of k, which at
@@ -323,7 +323,7 @@ int launch_typed(const I8Params& p, int num_sms, cudaStream_t stream) {
     cfg.numAttrs = 1;
     if (!clusters_of[dev & 63][1]) {
         CMFC_CUDA(cudaFuncSetAttribute(i8_pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
-        for (int s = MAX_SPLITS; s >= 1; s /= 2) {
+        for (int s = MAX_SPLITS; s >= 1; --s) {
             attr[0].val.clusterDim.x = 2 * s;
             cfg.gridDim = dim3(2 * s);
             int n = 0;
@@ -340,7 +340,7 @@ int launch_typed(const I8Params& p, int num_sms, cudaStream_t stream) {
     // K is cut while all tiles still run at once and a slice keeps at least four stages of work
     const int64_t tiles = tiles_m * tiles_n;
     pl.splits = 1;
-    for (int s = 2; s <= MAX_SPLITS; s *= 2)
+    for (int s = 2; s <= MAX_SPLITS; ++s)
         if (tiles <= clusters_of[dev & 63][s] && pl.kblocks >= 4 * s) pl.splits = s;
     const int es = (int)elem_bytes(p.out_elem);
     pl.tma_out = pl.splits == 1 && !(reinterpret_cast<uintptr_t>(p.y) & 15) && (p.ldy * es) % 16 == 0;
