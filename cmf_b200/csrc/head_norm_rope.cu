@@ -36,10 +36,10 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(NormRopeParams p, int he
     constexpr int V = 16 / sizeof(T);  // elements of a 16-byte chunk
     const int u = threadIdx.x % LANES;                 // this lane's unit: two chunks, V pairs
     const int units = p.hd / (2 * V), rot_units = p.rot / (2 * V);
-    const int64_t item = (int64_t)blockIdx.x * (128 / LANES) + threadIdx.x / LANES;
-    const bool active = u < units && item < p.n * items_per_token;
-    const int64_t t = active ? item / items_per_token : 0;
-    const int part = active ? (int)(item % items_per_token) : 0;
+    const uint32_t item = blockIdx.x * (128 / LANES) + threadIdx.x / LANES;  // fewer than 2^31
+    const bool active = u < units && item < (uint32_t)p.n * items_per_token;
+    const int64_t t = active ? item / (uint32_t)items_per_token : 0;
+    const int part = active ? (int)(item % (uint32_t)items_per_token) : 0;
     const bool is_q = part < q_items;
     const int head0 = (is_q ? part : part - q_items) * heads_per_item;
     const int heads = active ? min(heads_per_item, (is_q ? p.nh : p.nkv) - head0) : 0;
@@ -98,8 +98,8 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(NormRopeParams p, int he
                 b = rb;
             }
         }
-        *reinterpret_cast<uint4*>(dst + h * out.head + d0) = pack16<T>(x);
-        *reinterpret_cast<uint4*>(dst + h * out.head + d1) = pack16<T>(x + V);
+        __stcs(reinterpret_cast<uint4*>(dst + h * out.head + d0), pack16<T>(x));
+        __stcs(reinterpret_cast<uint4*>(dst + h * out.head + d1), pack16<T>(x + V));
     }
 }
 
