@@ -210,6 +210,7 @@ template <typename T, int TPR, int CH>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int rows, int chunks,
                                                                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
     constexpr int V = 16 / (int)sizeof(T);
+    let_product_start();
     const int64_t r = (int64_t)blockIdx.x * (QUANT_THREADS / TPR) + threadIdx.x / TPR;
     if (TPR == 32 && r >= rows) return;  // a whole warp
     const int t = threadIdx.x % TPR;
@@ -242,6 +243,7 @@ __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_kernel(const T* _
 template <typename T>
 __global__ void __launch_bounds__(QUANT_THREADS) quantize_rows_any_kernel(const T* __restrict__ x, int64_t ldx, int cols, int8_t* __restrict__ q,
                                                                           int64_t ldq, float* __restrict__ scale) {
+    let_product_start();
     const int64_t r = blockIdx.x;
     const T* src = x + r * ldx;
     int8_t* dst = q + r * ldq;

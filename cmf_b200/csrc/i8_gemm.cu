@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) i8_rows_kernel(I8Params p, co
     };
     int k0 = warp * 64;
     load_w(a[0], k0);
+    wait_for_quantizer();  // the weights do not depend on it
     if constexpr (FUSED) round_tokens<X>(p, act, ld_act, levels, scales, &red[0][0][0]);
     for (; k0 < (int)p.K; k0 += 2 * STEP) {  // the next piece of the weights is on its way while one is multiplied
         load_w(a[1], k0 + STEP);
@@ -176,10 +177,19 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) i8_rows_kernel(I8Params p, co
 }
 
 template <typename T>
-void launch_rows(const I8Params& p, cudaStream_t s) {
-    const unsigned blocks = (unsigned)((p.N + 15) / 16);
-    if (p.M <= 8) i8_rows_kernel<T, int8_t, 1><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p, nullptr, 0);
-    else i8_rows_kernel<T, int8_t, 2><<<blocks, 32 * ROWS_WARPS, 0, s>>>(p, nullptr, 0);
+cudaError_t launch_rows(const I8Params& p, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)((p.N + 15) / 16));
+    cfg.blockDim = dim3(32 * ROWS_WARPS);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.behind_quantizer ? 1 : 0;
+    const int8_t* none = nullptr;
+    if (p.M <= 8) return cudaLaunchKernelEx(&cfg, i8_rows_kernel<T, int8_t, 1>, p, none, (int64_t)0);
+    return cudaLaunchKernelEx(&cfg, i8_rows_kernel<T, int8_t, 2>, p, none, (int64_t)0);
 }
 
 template <typename T, typename X>
@@ -218,10 +228,7 @@ int launch_i8_matmat(const I8Params& p, int num_sms, cudaStream_t s) {
     const bool aligned = !((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) && p.ldx % 16 == 0 && p.ldw % 16 == 0;
     // 9 to 16 tokens: 4096 x 4096 weights 7.0 us here, 9.9 on CTA pairs; 2304 x 9216 11.5 and 11.3; 18432 x 2304 15.7 and 11.8
     if (aligned && p.M <= ROWS_MAX_TOKENS && p.K % 16 == 0 && (p.M <= 8 || p.N * p.K <= (int64_t)20 << 20)) {
-        if (p.out_elem == ET_F32) launch_rows<float>(p, s);
-        else if (p.out_elem == ET_F16) launch_rows<__half>(p, s);
-        else launch_rows<__nv_bfloat16>(p, s);
-        CMFC_CUDA(cudaGetLastError());
+        CMFC_CUDA(p.out_elem == ET_F32 ? launch_rows<float>(p, s) : p.out_elem == ET_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s));
         return OK;
     }
     if (aligned) return launch_i8_pair(p, num_sms, s);

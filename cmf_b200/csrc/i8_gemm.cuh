@@ -13,6 +13,11 @@ bool i8_fused_supported(const I8Params& p, const void* act, int elem, int64_t ld
 int launch_i8_fused(const I8Params& p, const void* act, int elem, int64_t ld_act, cudaStream_t s);
 
 #ifdef __CUDACC__
+// The product is launched while the quantizer in front of it still runs (programmatic stream serialization): it sets
+// itself up and then waits here until the quantizer is through.  Without that attribute the wait is over at once.
+__device__ __forceinline__ void wait_for_quantizer() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_product_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // A row's scale and levels from the largest bit pattern of its |x| (NaN above infinity above every number):
 // scale = max |x| / 127, level = rint(x / scale) (ties to even), both quotients IEEE f32.  Zeros, or a scale
 // that underflows to zero: scale 0, levels 0; an infinity or a NaN: scale NaN, levels 0.

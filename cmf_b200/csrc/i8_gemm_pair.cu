@@ -145,6 +145,7 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     cluster.sync();  // every barrier is initialised before anyone signals across the pair
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
+    wait_for_quantizer();
 
     if (warp == 0) {
         if (elect_one()) {
@@ -313,7 +314,9 @@ int launch_typed(const I8Params& p, int num_sms, cudaStream_t stream) {
     int dev = 0;
     CMFC_CUDA(cudaGetDevice(&dev));
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.blockDim = dim3(THREADS);
@@ -352,6 +355,7 @@ int launch_typed(const I8Params& p, int num_sms, cudaStream_t stream) {
     const int64_t most = pl.splits > 1 ? tiles : std::min<int64_t>(tiles, num_sms / 2);
     attr[0].val.clusterDim.x = 2 * pl.splits;
     cfg.gridDim = dim3((unsigned)(most * 2 * pl.splits));
+    cfg.numAttrs = p.behind_quantizer ? 2 : 1;
     CMFC_CUDA(cudaLaunchKernelEx(&cfg, i8_pair_kernel<T>, tm_x, tm_w, tm_y, p, pl));
     return OK;
 }

@@ -159,6 +159,7 @@ int i8_linear_impl(int device, const void* x, int elem, int64_t ldx, const int8_
     p.x = q;
     p.x_scale = scale;
     p.ldx = up16(cols);
+    p.behind_quantizer = 1;
     CMFC_TRY(launch_i8_matmat(p, on.c->num_sms, s));
     count_launches(on.c, 2);
     return OK;

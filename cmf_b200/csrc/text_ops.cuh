@@ -40,6 +40,7 @@ struct I8Params {
     int64_t M, N, K;
     int out_elem;
     uint32_t* status;
+    int behind_quantizer;  // the launch before this one on the stream is the quantizer of x: set up while it runs
 };
 int launch_i8_matmat(const I8Params& p, int num_sms, cudaStream_t s);
 
