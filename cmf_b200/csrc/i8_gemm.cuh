@@ -19,14 +19,16 @@ __device__ __forceinline__ void wait_for_quantizer() { asm volatile("griddepcont
 __device__ __forceinline__ void let_product_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // A row's scale and levels from the largest bit pattern of its |x| (NaN above infinity above every number):
-// scale = max |x| / 127, level = rint(x / scale) (ties to even), both quotients IEEE f32.  Zeros, or a scale
-// that underflows to zero: scale 0, levels 0; an infinity or a NaN: scale NaN, levels 0.
+// scale = max |x| * (1 / 127), the constant and the product each rounded to f32; level = rint(x / scale) (ties to
+// even), an IEEE f32 quotient.  The product is what torch computes for `x.abs().amax(1) / 127` on a CUDA tensor: x = max / 2
+// and every odd multiple of max / 254 that the type holds lie on a tie, so that a scale one unit off the caller's would
+// move their levels.  Zeros, or a scale that underflows to zero: scale 0, levels 0; an infinity or a NaN: scale NaN, levels 0.
 struct RowScale {
     float scale, inv;
     bool zero, slow;
     __device__ __forceinline__ explicit RowScale(unsigned top) {
         const bool finite = top < 0x7f800000u;
-        scale = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __int_as_float(0x7fc00000);
+        scale = finite ? __fmul_rn(__uint_as_float(top), 1.0f / 127.0f) : __int_as_float(0x7fc00000);
         zero = !finite || scale == 0.0f;
         slow = !(scale >= 1e-30f && scale <= 1e30f);  // the reciprocal could leave the normal numbers
         inv = __frcp_rn(scale);

@@ -42,10 +42,11 @@ def norm_rope(x, weight, cos, sin, half_split, eps=1e-5):
 
 
 def quantize_rows(x):
-    """The levels and scales bit for bit: both quotients are correctly rounded f32 divisions."""
+    """The levels and scales bit for bit: the scale is the f32 product with the f32 number next to 1 / 127, the levels
+    come from a correctly rounded f32 division."""
     x = x.float().cpu()
     top = x.abs().amax(1)
-    scale = top / torch.tensor(127.0)
+    scale = top * (torch.tensor(1.0) / torch.tensor(127.0))
     finite = torch.isfinite(x).all(1)
     safe = torch.where(finite & (scale > 0), scale, torch.ones_like(scale))
     q = torch.where((finite & (scale > 0))[:, None], x / safe[:, None], torch.zeros_like(x)).round().clamp(-127, 127).to(torch.int8)
