@@ -18,6 +18,9 @@ namespace {
 
 static_assert(CMFC_ET_F32 == ET_F32 && CMFC_ET_F16 == ET_F16 && CMFC_ET_BF16 == ET_BF16, "element types of the header");
 
+// counts stay a tile below 2^31, so that the end of the last tile is a number too
+constexpr size_t MOST = (size_t)INT_MAX - 1023;
+
 bool elem_ok(int e) { return e == ET_F32 || e == ET_F16 || e == ET_BF16; }
 
 // Makes `device` current for the launches of one entry and puts the caller's device back; the device's
@@ -71,7 +74,7 @@ int guarded(F f) {
 int quantize_rows_impl(int device, const void* x, int elem, size_t rows, size_t cols, int64_t ldx, int8_t* q, int64_t ldq,
                        float* scale, cudaStream_t s) {
     NEED(elem_ok(elem), "quantize_rows: unknown element type");
-    NEED(rows <= INT_MAX && cols >= 1 && cols <= INT_MAX, "quantize_rows: rows must be below 2^31, cols in [1, 2^31)");
+    NEED(rows <= MOST && cols >= 1 && cols <= MOST, "quantize_rows: rows must be at most 2^31 - 1024, cols in [1, 2^31 - 1024]");
     if (rows == 0) return OK;
     NEED(x && q && scale, "quantize_rows: null pointer");
     NEED(stride_ok(ldx) && stride_ok(ldq) && (rows == 1 || (ldx >= (int64_t)cols && ldq >= (int64_t)cols)),
@@ -104,7 +107,7 @@ I8Params i8_params(const int8_t* wq, int64_t ldw, const float* ws, size_t b, siz
 int i8_matmat_impl(int device, const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw, const float* ws,
                    size_t b, size_t rows, size_t cols, void* y, int elem, int64_t ldy, cudaStream_t s) {
     NEED(elem_ok(elem), "i8_matmat: unknown output type");
-    NEED(b <= INT_MAX && rows >= 1 && rows <= INT_MAX, "i8_matmat: b must be below 2^31, rows in [1, 2^31)");
+    NEED(b <= MOST && rows >= 1 && rows <= MOST, "i8_matmat: b must be at most 2^31 - 1024, rows in [1, 2^31 - 1024]");
     NEED(cols >= 1, "i8_matmat: cols must not be 0");
     if (cols > (size_t)I8_MAX_K) return fail(ERR_UNSUPPORTED, "i8_matmat: cols above 131071 could overflow the 32-bit sum");
     if (b == 0) return OK;
@@ -125,7 +128,7 @@ int i8_matmat_impl(int device, const int8_t* xq, int64_t ldx, const float* xs, c
 }
 
 size_t i8_linear_workspace(const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, size_t b, size_t rows, size_t cols) {
-    if (b > INT_MAX || cols > (size_t)I8_MAX_K || rows > INT_MAX || !elem_ok(elem)) return 0;  // refused by the call itself
+    if (b > MOST || cols > (size_t)I8_MAX_K || rows > MOST || !elem_ok(elem)) return 0;  // refused by the call itself
     const I8Params p = i8_params(wq, ldw, nullptr, b, rows, cols, nullptr, ET_F32, (int64_t)rows);
     return i8_fused_supported(p, x, elem, pitch(b, cols, ldx)) ? 0 : b * (size_t)up16(cols) + 4 * b;
 }
@@ -133,7 +136,7 @@ size_t i8_linear_workspace(const void* x, int elem, int64_t ldx, const int8_t* w
 int i8_linear_impl(int device, const void* x, int elem, int64_t ldx, const int8_t* wq, int64_t ldw, const float* ws, size_t b,
                    size_t rows, size_t cols, void* y, int y_elem, int64_t ldy, void* work, size_t work_bytes, cudaStream_t s) {
     NEED(elem_ok(elem) && elem_ok(y_elem), "i8_linear: unknown element type");
-    NEED(b <= INT_MAX && rows >= 1 && rows <= INT_MAX, "i8_linear: b must be below 2^31, rows in [1, 2^31)");
+    NEED(b <= MOST && rows >= 1 && rows <= MOST, "i8_linear: b must be at most 2^31 - 1024, rows in [1, 2^31 - 1024]");
     NEED(cols >= 1, "i8_linear: cols must not be 0");
     if (cols > (size_t)I8_MAX_K) return fail(ERR_UNSUPPORTED, "i8_linear: cols above 131071 could overflow the 32-bit sum");
     if (b == 0) return OK;
@@ -215,7 +218,7 @@ int window_attention_impl(int device, const cmfc_window_attention_args* a, cudaS
     NEED(a->hd >= 1, "window_attention: empty heads");
     if (a->hd > 256) return fail(ERR_UNSUPPORTED, "window_attention: head sizes above 256 are not implemented");
     NEED(isfinite(a->scale) && isfinite(a->softcap) && a->softcap >= 0.0f, "window_attention: scale and softcap must be finite, softcap not negative");
-    NEED(a->q_rows <= INT_MAX && a->k_rows <= INT_MAX && a->q_rows * (a->nh / a->nkv) <= INT_MAX, "window_attention: more than 2^31 rows");
+    NEED(a->q_rows <= MOST && a->k_rows <= MOST && a->q_rows * (a->nh / a->nkv) <= MOST, "window_attention: more than 2^31 - 1024 rows");
     const bool packed = a->q_start || a->k_start || a->k_len;
     NEED(!packed || (a->q_start && a->k_start && a->k_len), "window_attention: q_start, k_start and k_len come together");
     NEED(packed ? a->seqs <= 1u << 30 : a->seqs == 1, "window_attention: without q_start there is one sequence");

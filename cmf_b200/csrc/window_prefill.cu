@@ -36,7 +36,7 @@ template <int HDP> __host__ __device__ constexpr int q_tiles() { return HDP <= 1
 template <int HDP> __host__ __device__ constexpr int slots() { return HDP == 64 ? 12 : 10; }
 constexpr int THREADS = 32 * (2 + 8);
 template <int HDP> __host__ __device__ constexpr int q_bytes() { return QT * HDP * 2; }
-constexpr int BARS_BYTES = 3072;
+constexpr int BARS_BYTES = 3 * 1024;
 template <int HDP> __host__ __device__ constexpr int smem_bytes() { return q_tiles<HDP>() * q_bytes<HDP>() + slots<HDP>() * SLOT + BARS_BYTES; }
 
 struct Bars {
@@ -88,11 +88,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-
-// Soft cap.  Where all |y| = |score / cap| of a warp's rows are at most 0.75, tanh(y) = y P(y^2) on the FMA pipe, P of degree 5
-// fitted to tanh(sqrt z) / sqrt z on [0, 0.5625] at Chebyshev points (relative error 3e-8, 1.1e-7 with f32 roundings);
-// else 1 - 2 / (2^(2 y log2 e) + 1) on the special-function unit, which the exponentials of the softmax already fill.
-__device__ __forceinline__ float cap_tanh(float y) { return 1.0f - __fdividef(2.0f, ex2_approx(y * (2.0f * LOG2E)) + 1.0f); }
 
 // bit i: the row at position pos sees key j0 + i
 __device__ __forceinline__ uint32_t seen_bits(const WindowAttnParams& p, int pos, int j0) {
@@ -312,7 +307,8 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         const int pos = live ? shift + qi : -1;
         const uint32_t s_at = tmem + lane_addr + x * 128, o_at = tmem + lane_addr + o_col + (two ? x * 128 : 0);
         const float c = p.scale * LOG2E, cap2 = p.softcap * LOG2E, to_y = CAP ? p.scale / p.softcap : 0.0f;
-        // P's coefficients for a score s instead of y = s to_y, times cap log2(e)
+        // Soft cap: where all scores of a warp's rows lie in cap_tanh's polynomial range, its coefficients for a score s instead
+        // of y = s to_y, times cap log2(e), leave seven packed instructions for the exponents of two scores
         float cap_c[6] = {1.0f, -0.3333296776f, 0.1332551539f, -0.0533498190f, 0.0195937864f, -0.0047239522f};
         if (CAP) {
             float f = cap2 * to_y;
@@ -361,7 +357,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
                         mns[(i >> 1) & 3] = fminf(mns[(i >> 1) & 3], fminf(__uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1])));
-                small = __all_sync(0xffffffffu, fmaxf(mx, -fminf(fminf(mns[0], mns[1]), fminf(mns[2], mns[3]))) * to_y <= 0.75f);
+                small = __all_sync(0xffffffffu, to_y <= 1e3f && fmaxf(mx, -fminf(fminf(mns[0], mns[1]), fminf(mns[2], mns[3]))) * to_y <= TANH_POLY_MAX);
             }
             // the cap keeps the order: the largest capped score is the capped largest score
             const float m_cand = !CAP ? mx * c : mx == -INFINITY ? mx : cap2 * cap_tanh(mx * to_y);

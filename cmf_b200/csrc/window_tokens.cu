@@ -151,7 +151,7 @@ window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             for (int k = 0; k < HDP / 16; ++k) ldsm4(qf[k], qa + k * 32);
         }
         const int pos0 = g < rows ? shift + (r0 + g) / group : -1, pos1 = g + 8 < rows ? shift + (r0 + g + 8) / group : -1;
-        const float sc = p.scale * LOG2E, cap2 = p.softcap * LOG2E, two_y = CAP ? 2.0f * sc / p.softcap : 0.0f;
+        const float sc = p.scale * LOG2E, cap2 = p.softcap * LOG2E, to_y = CAP ? p.scale / p.softcap : 0.0f;
         const int pos_min = shift + first_i, seen_last = shift + last_i;
         const int seen_low = (int)max((int64_t)0, (int64_t)pos_min - p.window + 1);
         auto ready = [&](int t) {
@@ -200,12 +200,12 @@ window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             scores(stage_at(more ? t + L::TEAMS : t), nxt);
             const int j0 = kt.at(t) * KEYS + half * 16;
             const uint32_t vs = stage_at(t) + L::KTILE;
-            float x[2][4];  // log2 units; cap tanh(y) = cap (1 - 2 / (e^2y + 1))
+            float x[2][4];  // log2 units
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    x[n][e] = CAP ? cap2 - __fdividef(2.0f * cap2, ex2_approx(cur[n][e] * two_y) + 1.0f) : cur[n][e] * sc;
+                    x[n][e] = CAP ? cap2 * cap_tanh(cur[n][e] * to_y) : cur[n][e] * sc;
             if (j0 + 15 > pos_min || ((int64_t)seen_last - j0 >= p.window && j0 + 16 > p.sinks)) {  // some row does not see all 16 keys
 #pragma unroll
                 for (int n = 0; n < 2; ++n)

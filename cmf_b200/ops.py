@@ -14,6 +14,7 @@ import struct
 from ._lib import CmfCudaError, check, lib
 
 _BAD_ARG, _UNSUPPORTED, _SHAPE = -1, -2, -3
+_ALL = 2 ** 31 - 1  # no sequence is longer
 # the argument structs of include/cmf_cuda.h in the platform's own layout
 _ROPE = struct.Struct("@9P8q2Q4I3if")    # cmfc_qk_norm_rope_args
 _ATTN = struct.Struct("@7P8q4Q4I2fi4x")  # cmfc_window_attention_args
@@ -91,9 +92,10 @@ def _rows(name, t):
 
 
 def quantize_rows(x):
-    """Rows to 8 bits: ``scale = max |x| / 127`` and ``q = rint(x / scale)`` for each row of ``x`` [b, cols].
-    Returns ``(q, scale)``, int8 [b, cols] and float32 [b].  A row of zeros gives scale 0; a row that holds an
-    infinity or a NaN gives scale NaN and levels 0."""
+    """Rows to 8 bits: ``scale = max |x| / 127`` (times the f32 number next to 1 / 127, as torch divides a CUDA
+    tensor by a number) and ``q = rint(x / scale)`` for each row of ``x`` [b, cols].  Returns ``(q, scale)``, int8
+    [b, cols] and float32 [b].  A row of zeros gives scale 0; a row that holds an infinity or a NaN gives scale
+    NaN and levels 0."""
     if _torch is None:
         _load()
     ldx, elem = _rows("x", x), _elem("x", x)
@@ -268,10 +270,10 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, softcap=0.0, q_s
         _fail(_SHAPE, f"window_attention: {nh} query heads over {nkv} key heads of {hd}")
     if window is None:
         window = 0
-    elif window < 1:
-        _fail(_BAD_ARG, "window must be at least 1 (a query's own key), or None")
-    if sinks < 0:
-        _fail(_BAD_ARG, "sinks must not be negative")
+    elif window < 1 or int(window) != window:
+        _fail(_BAD_ARG, "window must be a whole number of at least 1 (a query's own key), or None")
+    if sinks < 0 or int(sinks) != sinks:
+        _fail(_BAD_ARG, "sinks must be a whole number and not negative")
     tensors = [q, k, v]
     seqs, qs, ks, kl = 1, 0, 0, 0
     if q_start is not None or k_start is not None or k_len is not None:
@@ -297,6 +299,6 @@ def window_attention(q, k, v, window=None, sinks=0, scale=None, softcap=0.0, q_s
     if rows == 0 or seqs == 0:
         return out
     args = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, kl, q_row, q_head, k_row, k_head, v_row, v_head,
-                      o_row, o_head, rows, krows, window, sinks, seqs, nh, nkv, hd, hd ** -0.5 if scale is None else scale, softcap, elem)
+                      o_row, o_head, rows, krows, min(int(window), _ALL), min(int(sinks), _ALL), seqs, nh, nkv, hd, hd ** -0.5 if scale is None else scale, softcap, elem)
     check(lib().cmfc_window_attention(dev, args, _stream(dev)))
     return out

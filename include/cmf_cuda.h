@@ -287,14 +287,15 @@ int cmfc_matmat_device_noalloc(cmfc_model* m, int64_t idx, const float* d_x, siz
 #define CMFC_ET_F16 1
 #define CMFC_ET_BF16 2
 
-/* Rows to 8 bits: scale[r] = max_c |x[r, c]| / 127, q[r, c] = rint(x[r, c] / scale[r]) (ties to even; both
- * quotients in f32).  A row of zeros gives scale 0 and levels 0; a row that holds an infinity or a NaN gives
+/* Rows to 8 bits: scale[r] = max_c |x[r, c]| * (1 / 127), q[r, c] = rint(x[r, c] / scale[r]) (ties to even;
+ * the constant, the product and the quotient each rounded to f32).  A row of zeros gives scale 0 and levels 0; a row that holds an infinity or a NaN gives
  * scale NaN and levels 0.  x [rows, cols] of type `elem`, pitch ldx; q pitch ldq; scale [rows]. */
 int cmfc_quantize_rows(int device, const void* x, int elem, size_t rows, size_t cols, int64_t ldx, int8_t* q, int64_t ldq,
                        float* scale, void* stream);
 /* y[m, n] = (sum_k xq[m, k] wq[n, k]) * (x_scale[m] * w_scale[n]): xq [b, cols], wq [rows, cols] (a q8_row
  * tensor's levels and row scales), y [b, rows] of type `elem`.  The sum is exact in 32-bit integers
- * (cols <= 131071).  Fastest with pitches and bases that are multiples of 16 bytes. */
+ * (cols <= 131071).  Fastest with pitches and bases that are multiples of 16 bytes (without: at most 4194240
+ * tokens). */
 int cmfc_i8_matmat(int device, const int8_t* xq, int64_t ldx, const float* x_scale, const int8_t* wq, int64_t ldw,
                    const float* w_scale, size_t b, size_t rows, size_t cols, void* y, int elem, int64_t ldy, void* stream);
 /* The two in one call: x [b, cols] of type `elem` through 8-bit weights, the same bits as cmfc_quantize_rows and

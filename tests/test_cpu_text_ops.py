@@ -60,6 +60,8 @@ def test_window_attention_refuses():
     refused(-1, attn, window=0)
     refused(-1, attn, window=-5)
     refused(-1, attn, sinks=-1)
+    refused(-1, attn, window=2.5)
+    refused(-1, attn, sinks=0.5)
     refused(-1, attn, q_start=i32(0, 4))
     refused(-3, attn, q_start=i32(0, 4), k_start=i32(0, 0), k_len=i32(4))
     refused(-3, attn, q_start=i32(0, 2, 4), k_start=i32(0), k_len=i32(4))
@@ -119,7 +121,7 @@ def test_library_refuses_before_any_device_call():
 
     for kw, code in [(dict(elem=-1), -1), (dict(nh=3), -1), (dict(nkv=0), -1), (dict(hd=0), -1), (dict(hd=257), -2), (dict(scale=float("inf")), -1),
                      (dict(softcap=-1.0), -1), (dict(seqs=2), -1), (dict(ptrs=[256] * 4 + [256, 0, 0]), -1), (dict(ptrs=[0] * 7), -1),
-                     (dict(q_rows=2 ** 31), -1), (dict(strides=[64, 16, 32, 16, 32, 16, 64, 8]), -1),
+                     (dict(q_rows=2 ** 31), -1), (dict(k_rows=2 ** 31 - 100), -1), (dict(q_rows=2 ** 30), -1), (dict(strides=[64, 16, 32, 16, 32, 16, 64, 8]), -1),
                      (dict(strides=[64, 16, 32, -16, 32, 16, 64, 16]), -1)]:
         assert L.cmfc_window_attention(0, attn_args(**kw), None) == code, (kw, L.cmfc_last_error())
     assert L.cmfc_window_attention(0, None, None) == -1
@@ -127,7 +129,7 @@ def test_library_refuses_before_any_device_call():
 
     q = lambda **kw: L.cmfc_quantize_rows(*{**dict(dev=0, x=p, elem=0, rows=4, cols=8, ldx=8, q=p, ldq=8, s=p, st=None), **kw}.values())  # noqa: E731
     assert q(elem=9) == -1 and q(cols=0) == -1 and q(x=None) == -1 and q(ldx=7) == -1 and q(ldq=7) == -1 and q(ldx=-8) == -1
-    assert q(rows=0) == 0
+    assert q(rows=0) == 0 and q(rows=2 ** 31 - 1) == -1 and q(cols=2 ** 31, ldx=2 ** 31, ldq=2 ** 31) == -1
     m = lambda **kw: L.cmfc_i8_matmat(*{**dict(dev=0, x=p, ldx=8, xs=p, w=p, ldw=8, ws=p, b=4, rows=4, cols=8, y=p, elem=0, ldy=4, st=None),  # noqa: E731
                                         **kw}.values())
     assert m(elem=9) == -1 and m(rows=0) == -1 and m(cols=0) == -1 and m(w=None) == -1 and m(ldx=7) == -1 and m(ldy=3) == -1

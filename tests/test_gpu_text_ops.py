@@ -279,12 +279,13 @@ def test_single_tokens_over_a_cache(nh, nkv, hd, window, sinks, cap, dtype):
     ref.check(out, *ref.window_attention(q, k, v, lens, starts, total, window or 1 << 30, sinks, hd ** -0.5, cap))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("nh,nkv,hd", [(8, 4, 256), (6, 2, 96), (4, 4, 64)])
-def test_many_single_tokens_over_long_caches(nh, nkv, hd):
+def test_many_single_tokens_over_long_caches(nh, nkv, hd, dtype):
     """Enough blocks and tiles that every ring wraps many times under load; each call gives the first one's bits."""
     from cmf_b200 import ops
     prior = [4095 - 61 * i for i in range(48)]
-    q, k, v, starts, total, where = attn_inputs([1] * 48, prior, nh, nkv, hd, torch.bfloat16, slots=4096)
+    q, k, v, starts, total, where = attn_inputs([1] * 48, prior, nh, nkv, hd, dtype, slots=4096)
     first = ops.window_attention(q, k, v, sinks=2, **where)
     ref.check(first, *ref.window_attention(q, k, v, [1] * 48, starts, total, 1 << 30, 2, hd ** -0.5, 0.0))
     outs = [ops.window_attention(q, k, v, sinks=2, **where) for _ in range(200)]
@@ -385,6 +386,34 @@ def test_large_scores_and_rising_maxima(dtype):
         k[:, :, 0] = torch.linspace(0, 200, k.shape[0], device="cuda")[:, None].to(dtype)
         out = ops.window_attention(q, k, v, window=250, sinks=5, scale=1.0)
         ref.check(out, *ref.window_attention(q, k, v, [n], [0], [400], 250, 5, 1.0, 0.0))
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 4, 256), (6, 2, 96), (4, 4, 64), (4, 1, 128)])
+def test_many_prompt_tiles_give_the_same_bits(nh, nkv, hd):
+    """Prompts and chunks over enough blocks and key tiles that every ring wraps many times, again and again."""
+    from cmf_b200 import ops
+    lens, prior = [700, 33, 1500, 129, 64], [900, 0, 300, 2000, 5]
+    q, k, v, starts, total, where = attn_inputs(lens, prior, nh, nkv, hd, torch.bfloat16)
+    first = ops.window_attention(q, k, v, window=1100, sinks=3, softcap=20.0, **where)
+    ref.check(first, *ref.window_attention(q, k, v, lens, starts, total, 1100, 3, hd ** -0.5, 20.0))
+    outs = [ops.window_attention(q, k, v, window=1100, sinks=3, softcap=20.0, **where) for _ in range(100)]
+    assert all(torch.equal(o, first) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 3.0, 1e4, 1e9])
+def test_caps_far_below_and_above_the_scores(dtype, cap):
+    """Scores of several units under a cap that they all reach, that some reach, and that none comes near."""
+    from cmf_b200 import ops
+    for nh, nkv, hd, n in ((4, 2, 64, 200), (2, 1, 256, 150), (4, 2, 128, 1), (4, 2, 256, 1)):
+        q, k, v, _, _, _ = attn_inputs([n], [260 - n], nh, nkv, hd, dtype)
+        out = ops.window_attention(q * 3, k, v, window=200, softcap=cap)
+        want, tol = ref.window_attention(q * 3, k, v, [n], [0], [260], 200, 0, hd ** -0.5, cap)
+        if cap > 1e3:  # the cap changes nothing: the tolerance that grows with it has to hold without it too
+            want, tol = ref.window_attention(q * 3, k, v, [n], [0], [260], 200, 0, hd ** -0.5, 0.0)
+            # y P(y^2) or tanhf: 6 roundings of a score of at most 3 x 1.5 x 6 x 6 = 162
+            tol = tol + 2 * 6 * 162 * ref.F32 * v.double().abs().max()
+        ref.check(out, want, tol)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -537,6 +566,70 @@ def test_calls_on_other_streams_in_two_graphs_and_at_once():
     for outs in got + [o for _, o in graphs]:
         for x1, x2 in zip(outs, want):
             assert torch.equal(x1, x2)
+
+
+CAPTURE = """
+import torch
+from cmf_b200 import ops
+x = torch.randn(40, 4, 64, device="cuda")
+ops.quantize_rows(x[:, 0])                     # the device's context exists; no other kernel has run yet
+torch.cuda.synchronize()
+w, s = torch.randint(-9, 9, (64, 256), device="cuda", dtype=torch.int8), torch.ones(64, device="cuda")
+def calls():
+    out = []
+    for t in (torch.float32, torch.float16, torch.bfloat16):
+        for y in (x.to(t), x.to(t)[..., :20]):
+            out.append(ops.window_attention(y, y[:, :2], y[:, 2:], window=9, softcap=5.0))
+            out.append(ops.window_attention(y[:1], y[:, :2], y[:, 2:]))
+        out += [ops.i8_linear(x.to(t).view(40, 256)[:b], w, s) for b in (1, 12, 40)]
+        out += ops.qk_norm_rope(x.to(t), None, s, None, x[:, 0, :32].contiguous(), x[:, 1, :32].contiguous())[:1]
+    return out
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(got, calls()):
+    assert torch.equal(a, b)
+print("captured")
+"""
+
+
+def test_first_launches_may_be_captured():
+    """A process whose first call of most kernels is inside a capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_the_first_call_on_a_device_is_refused_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from cmf_b200 import CmfCudaError, ops
+x = torch.ones(4, 64, device="cuda")
+torch.cuda.synchronize()
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            ops.quantize_rows(x)
+            code = 0
+        except CmfCudaError as e:
+            code = e.code
+        x.add_(1)
+finally:
+    print("code", code)
+q, s = ops.quantize_rows(x)
+torch.cuda.synchronize()
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "code -" in r.stdout, r.stdout + r.stderr[-2000:]
 
 
 def test_the_status_word_is_clear_and_launches_are_counted():
