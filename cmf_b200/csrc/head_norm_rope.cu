@@ -144,9 +144,11 @@ __global__ void __launch_bounds__(128) norm_rope_any_kernel(NormRopeParams p) {
 
 template <typename T, bool HALF, int LANES>
 void norm_rope_lanes(const NormRopeParams& p, cudaStream_t s) {
-    // few tokens: a head per lane group, so that the heads spread over the SMs (one token of 24 + 8
-    // heads); many: four heads share the gain and the rotation that a group holds in registers
-    const int per = p.n * (p.nh + p.nkv) >= 16384 ? HEADS_PER_ITEM : 1;
+    // few values: a head per lane group, so that the heads spread over the SMs; many: four heads share the gain and the
+    // rotation that a group holds in registers.  us, one / four (heads of 96, 32 of them, bf16): 1 token 2.2 / 3.1, 300
+    // tokens 3.3 / 3.9, 512 tokens 4.6 / 4.0, 8704 tokens 47 / 27; heads of 256, 12 of them: 300 tokens 3.2 / 3.6, 512
+    // tokens 4.3 / 4.2, 1000 tokens 6.4 / 4.8
+    const int per = p.n * (p.nh + p.nkv) * p.hd >= (int64_t)5 << 18 ? HEADS_PER_ITEM : 1;
     const int q_items = (p.nh + per - 1) / per, items = q_items + (p.nkv + per - 1) / per;
     const int64_t groups = p.n * items, per_block = 128 / LANES;
     norm_rope_kernel<T, HALF, LANES><<<(unsigned)((groups + per_block - 1) / per_block), 128, 0, s>>>(p, per, q_items, items);
@@ -268,9 +270,10 @@ void quantize_rows_typed(const void* x, int64_t rows, int64_t cols, int64_t ldx,
     const int chunks = (int)(cols / V);
     if (!vec) {
         quantize_rows_any_kernel<T><<<(unsigned)rows, QUANT_THREADS, 0, s>>>(xt, ldx, (int)cols, q, ldq, scale);
-    } else if (chunks <= 32 * 16 && rows >= 512) {
-        // a warp per row keeps up to 16 chunks in registers and needs no block barrier; with few rows a block per
-        // row spreads them over more SMs
+    } else if (chunks <= 32 * 16 && rows >= (chunks <= 32 * 4 ? 768 : 2560)) {
+        // a warp per row keeps up to 16 chunks a lane in registers and needs no block barrier; with few rows a block per row
+        // has more loads under way.  us, warp / block (bf16): 1024 columns 512 rows 2.4 / 2.2, 800 rows 2.4 / 2.5, 8704 rows 6.2
+        // / 12.8; 2304 columns 800 rows 3.8 / 2.9, 1600 rows 4.8 / 4.2, 8704 rows 13.9 / 17.6
         const unsigned blocks = (unsigned)((rows + 7) / 8);
         if (chunks <= 32 * 4) quantize_rows_kernel<T, 32, 4><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);
         else if (chunks <= 32 * 8) quantize_rows_kernel<T, 32, 8><<<blocks, QUANT_THREADS, 0, s>>>(xt, ldx, (int)rows, chunks, q, ldq, scale);

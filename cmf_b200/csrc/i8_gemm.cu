@@ -226,7 +226,8 @@ int launch_i8_fused(const I8Params& p, const void* act, int elem, int64_t ld_act
 
 int launch_i8_matmat(const I8Params& p, int num_sms, cudaStream_t s) {
     const bool aligned = !((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 15) && p.ldx % 16 == 0 && p.ldw % 16 == 0;
-    // 9 to 16 tokens: 4096 x 4096 weights 7.0 us here, 9.9 on CTA pairs; 2304 x 9216 11.5 and 11.3; 18432 x 2304 15.7 and 11.8
+    // us here / on CTA pairs (rows x columns of the weights): 1 token 2304 x 2304 2.9 / 7.2, 18432 x 2304 11.1 / 11.9; 8 tokens
+    // 2304 x 9216 9.1 / 11.3, 18432 x 2304 11.9 / 11.9; 16 tokens 4096 x 4096 6.9 / 9.9, 2304 x 9216 11.7 / 11.3, 18432 x 2304 15.8 / 12.1
     if (aligned && p.M <= ROWS_MAX_TOKENS && p.K % 16 == 0 && (p.M <= 8 || p.N * p.K <= (int64_t)20 << 20)) {
         CMFC_CUDA(p.out_elem == ET_F32 ? launch_rows<float>(p, s) : p.out_elem == ET_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s));
         return OK;

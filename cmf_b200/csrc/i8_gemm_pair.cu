@@ -340,11 +340,13 @@ int launch_typed(const I8Params& p, int num_sms, cudaStream_t stream) {
     pl.tiles_n = (int)tiles_n;
     pl.tt = (int)((((p.M + tiles_m - 1) / tiles_m) + 31) / 32 * 32);
     pl.kblocks = (int)((p.K + BK - 1) / BK);
-    // K is cut while all tiles still run at once and a slice keeps at least four stages of work
+    // K is cut as far as all tiles still run at once.  Joining the slices costs 2 us with few tokens a tile and 5 with many, a
+    // stage of work 0.2 us.  us, cut / whole (tokens x weight rows x columns): 32 x 2304 x 1024 7.0 / 6.2, x 2304 7.4 / 7.6, x 9216
+    // 11.4 / 19.2; 333 x 2304 x 2304 12.0 / 11.1, x 3456 12.9 / 13.3, x 9216 17.0 / 23.4; 512 x 2304 x 2304 13.8 / 12.9, x 9216 20.2 / 28.6
     const int64_t tiles = tiles_m * tiles_n;
     pl.splits = 1;
     for (int s = 2; s <= MAX_SPLITS; ++s)
-        if (tiles <= clusters_of[dev & 63][s] && pl.kblocks >= 4 * s) pl.splits = s;
+        if (tiles <= clusters_of[dev & 63][s] && pl.kblocks >= 10 + pl.tt / 16) pl.splits = s;
     const int es = (int)elem_bytes(p.out_elem);
     pl.tma_out = pl.splits == 1 && !(reinterpret_cast<uintptr_t>(p.y) & 15) && (p.ldy * es) % 16 == 0;
     CUtensorMap tm_x, tm_w, tm_y;

@@ -1,6 +1,6 @@
 // Causal attention with a sliding window and first tokens that stay visible, over packed sequences or
-// caches, any head size up to 256, any stride, f32 / f16 / bf16: the form for every call that the
-// tensor-core kernels (window_prefill.cu, window_tokens.cu) do not take, and the one for f32 prompts.
+// caches, any head size up to 256, any stride, f32 / f16 / bf16: the form for calls whose rows are not 16-byte
+// aligned.  The others go to window_prefill.cu, window_tokens.cu and window_f32.cu.
 //
 //   query i of a sequence with Lq queries and Lk keys stands at position p = Lk - Lq + i and sees key j
 //   when j <= p and (p - j < window or j < sinks);   s = scale q.k (soft cap: s = cap tanh(s / cap));
@@ -201,10 +201,9 @@ int launch_window_any(const WindowAttnParams& p, int elem, cudaStream_t s) {
 }
 
 int launch_window_attention(const WindowAttnParams& p, int elem, int num_sms, cudaStream_t s) {
-    // up to 32 rows a sequence on average: the key axis is what there is to split
-    if (p.q_rows * (p.nh / p.nkv) <= 32 * (int64_t)p.seqs && window_tokens_supported(p, elem)) return launch_window_tokens(p, elem, num_sms, s);
+    if (window_few_rows(p, num_sms) && window_tokens_supported(p, elem)) return launch_window_tokens(p, elem, num_sms, s);
     if (window_prefill_supported(p, elem)) return launch_window_prefill(p, elem, s);
-    if (window_f32_supported(p, elem)) return launch_window_f32(p, s);
+    if (window_f32_supported(p, elem)) return launch_window_f32(p, num_sms, s);
     return launch_window_any(p, elem, s);
 }
 

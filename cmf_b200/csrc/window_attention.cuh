@@ -10,7 +10,7 @@ int launch_window_any(const WindowAttnParams& p, int elem, cudaStream_t s);
 bool window_prefill_supported(const WindowAttnParams& p, int elem);
 int launch_window_prefill(const WindowAttnParams& p, int elem, cudaStream_t s);
 bool window_f32_supported(const WindowAttnParams& p, int elem);
-int launch_window_f32(const WindowAttnParams& p, cudaStream_t s);
+int launch_window_f32(const WindowAttnParams& p, int num_sms, cudaStream_t s);
 bool window_tokens_supported(const WindowAttnParams& p, int elem);
 int launch_window_tokens(const WindowAttnParams& p, int elem, int num_sms, cudaStream_t s);
 
@@ -26,6 +26,19 @@ inline int64_t window_items(const WindowAttnParams& p, int rows_per_tile) {  // 
 }
 inline int64_t window_range(const WindowAttnParams& p) {  // keys of a row
     return std::min<int64_t>((int64_t)p.window + p.sinks, std::max<int64_t>(1, p.k_rows / p.seqs));
+}
+
+// Few rows: the single-token kernels (tiles of 4 or 16 rows, the key axis cut); many: the prompt kernels (tiles of 64 or 128
+// rows over all keys).  A prompt tile costs the same for one row as for all, so the former win up to 16 rows a sequence, and
+// longer where 16-row tiles are no more than the SMs: there prompt tiles leave most of them idle.  us, single-token kernel / prompt kernel:
+//                                            bf16                          f32
+//   sequences x key heads x dims x keys      16 rows   24 rows   128 rows  16 rows     24 rows     128 rows
+//   64 x 8 x 128 x 2048                      94 / 122  136 / 123 442 / 130 626 / 1151  928 / 1152  4737 / 2000
+//   64 x 4 x 256 x 1024                      63 / 60   96 / 60   338 / 68  440 / 534   688 / 535   3481 / 1074
+//   8 x 8 x 64 x 4096                        18 / 47   25 / 47   79 / 40   130 / 368   228 / 368   882 / 608
+//   1 x 8 x 128 x 8192                       16 / 93   22 / 93   35 / 91   58 / 1139   76 / 1139   397 / 1141
+inline bool window_few_rows(const WindowAttnParams& p, int num_sms) {
+    return p.q_rows * (p.nh / p.nkv) <= 16 * (int64_t)p.seqs || window_items(p, 16) <= num_sms;
 }
 
 #ifdef __CUDACC__

@@ -428,18 +428,18 @@ int launch_tokens(const WindowAttnParams& p, cudaStream_t s) {
             clusters_of[dev & 63][n] = active > 0 ? active : 1;
         }
     }
-    // as for the 16-bit types (window_tokens.cu): cut only while all shares run at once and keep two key tiles
+    // As for the 16-bit types (window_tokens.cu): cut only while all shares run at once, and keep a key tile each (one
+    // sequence x 8 heads of 128 x 256 / 512 keys: 7.6 / 7.8 us, with two tiles each 9.1 / 9.5, with eight 12.7 / 21.8).
     int splits = 1;
-    while (splits < MAX_SPLITS && window_items(p, TR) <= clusters_of[dev & 63][2 * splits] && window_range(p) / (2 * splits) >= 2 * BN) splits *= 2;
+    while (splits < MAX_SPLITS && window_items(p, TR) <= clusters_of[dev & 63][2 * splits] && window_range(p) / (2 * splits) >= BN) splits *= 2;
     attr[0].val.clusterDim.x = splits;
     cfg.gridDim = dim3((unsigned)(max_tiles(p, TR) * p.nkv * splits));
     CMFC_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, splits));
     return OK;
 }
 template <int HDP>
-int launch_hdp(const WindowAttnParams& p, cudaStream_t s) {
-    // up to 32 rows a sequence on average: the key axis is what there is to split
-    if (p.q_rows * (p.nh / p.nkv) <= 32 * (int64_t)p.seqs) return launch_tokens<HDP>(p, s);
+int launch_hdp(const WindowAttnParams& p, int num_sms, cudaStream_t s) {
+    if (window_few_rows(p, num_sms)) return launch_tokens<HDP>(p, s);
     return launch_prompts<HDP>(p, s);
 }
 
@@ -450,10 +450,10 @@ bool window_f32_supported(const WindowAttnParams& p, int elem) {
     return elem == ET_F32 && p.hd % 4 == 0 && max_tiles(p, TR) * p.nkv * MAX_SPLITS < ((int64_t)1 << 31) && fits(p.q) && fits(p.k) && fits(p.v);
 }
 
-int launch_window_f32(const WindowAttnParams& p, cudaStream_t s) {
-    if (p.hd <= 64) return launch_hdp<64>(p, s);
-    if (p.hd <= 128) return launch_hdp<128>(p, s);
-    return launch_hdp<256>(p, s);
+int launch_window_f32(const WindowAttnParams& p, int num_sms, cudaStream_t s) {
+    if (p.hd <= 64) return launch_hdp<64>(p, num_sms, s);
+    if (p.hd <= 128) return launch_hdp<128>(p, num_sms, s);
+    return launch_hdp<256>(p, num_sms, s);
 }
 
 }  // namespace cmfc
