@@ -10,7 +10,9 @@
 // are read once per (token, up to HEADS_PER_ITEM heads) and stay in registers.  A lane owns two
 // 16-byte chunks of a head that hold both members of its pairs (neighbouring chunks, or the same
 // chunk of either half), so the rotation needs no exchange between lanes; a head takes a group of
-// 4 to 32 lanes and a warp works on 32 / group items.
+// 4 to 32 lanes and a warp works on 32 / group items.  Measured, 8704 tokens x 32 heads of 96: f32 37 us (5.9 TB/s, 0.90 of a
+// copy's rate); bf16 27 us (4.1 TB/s), where the conversions and the reduction of 32 values a lane hold up the loads; one
+// token 2.2 us.  Items by a 2-D grid, a loop over tokens and a register cap were each slower.
 #include "i8_gemm.cuh"
 
 namespace cmfc {
@@ -182,7 +184,8 @@ void norm_rope_typed(const NormRopeParams& p, cudaStream_t s) {
 
 // ---------------- rows to 8 bits ----------------
 // Bound: memory, the activations once and the levels once.  A row is read once into registers by a warp (short rows)
-// or a block of 256 threads, CH 16-byte chunks a thread; what does not fit is read again, from L2.
+// or a block of 256 threads, CH 16-byte chunks a thread; what does not fit is read again, from L2.  Measured, bf16, 8704 rows:
+// 2304 columns 13.9 us (4.3 TB/s), 9216 columns 48 us (5.0 TB/s); f32, 2304 columns 21 us (4.7 TB/s).
 constexpr int QUANT_THREADS = 256;
 
 // top of the bit patterns of |x| over a chunk, NaN above infinity above every number; 16-bit types two at a time

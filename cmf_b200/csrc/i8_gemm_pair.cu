@@ -15,7 +15,8 @@
 // stages' own space.  Integer sums are exact, so neither the cut nor the batch changes a bit of the result.
 //
 // Bound: the tensor pipe, and close behind it L2 -> SM (a 256 x 256 tile takes 64 KB per 128 levels of k, which at
-// the full 8-bit rate is near the 64 bytes a clock that an SM can take).
+// the full 8-bit rate is near the 64 bytes a clock that an SM can take).  Measured, bf16 out: 8704 x 18432 x 2304 244 us =
+// 3030 TOP/s, 0.92 of twice the bf16 rate of a library product.
 #include <cooperative_groups.h>
 
 #include <algorithm>

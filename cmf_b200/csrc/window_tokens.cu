@@ -10,6 +10,9 @@
 //               behind the other
 //   other warps 16 keys at a time each, teams of one or two warps taking tiles in turn: S = Q K^T by m16n8k16 (rows of
 //               queries beside each other, f32 sums), mask, soft cap, running maximum, exp2, O += P V
+// Measured, bf16: 64 sequences x 4096 keys x 4 heads of 256 165 us, x 8 heads of 128 167 us (6.5 TB/s, a copy's rate); one
+// sequence x 131072 keys x 8 heads of 128 115 us (4.7 TB/s); one sequence x 1000 keys 10 us, of which 5 are the launch of the
+// cluster, its joining and the way of the first tile.
 // Rows of V that no row of the block sees are zeroed in shared memory first (0 x NaN), and rows whose result is not
 // finite are computed again key by key (redo_row).
 #include <cooperative_groups.h>

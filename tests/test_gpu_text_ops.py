@@ -416,6 +416,62 @@ def test_caps_far_below_and_above_the_scores(dtype, cap):
         ref.check(out, want, tol)
 
 
+def with_rows_behind(monkeypatch):
+    """window_attention with so many rows behind the last sequence that a call goes to the kernels for prompts, whose
+    choice goes by the tensors' sizes; strides and alignment stay as they were."""
+    from cmf_b200 import ops
+    plain = ops.window_attention
+
+    def longer(t, rows):
+        nh, hd = t.shape[1:]
+        row, head = t.stride(0), t.stride(1)
+        head = rows * row if head >= row else head  # heads before tokens
+        skip = t.data_ptr() % 16 // t.element_size()
+        at = torch.full((skip + rows * row + nh * head + hd,), 7.0, dtype=t.dtype, device=t.device)
+        u = at.as_strided((rows, nh, hd), (row, head, 1), skip)
+        u[:t.shape[0]] = t
+        return u
+
+    def call(q, k, v, q_start=None, k_start=None, k_len=None, out=None, **kw):
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+        n = q.shape[0]
+        if n == 0:
+            return plain(q, k, v, **kw)
+        if q_start is None:
+            q_start, k_start, k_len = i32(0, n), i32(0), i32(k.shape[0])
+        rows = n + 2400 * len(k_start) * k.shape[1] // q.shape[1]
+        o = longer(torch.empty_like(q) if out is None else out, rows)
+        plain(longer(q, rows), k, v, q_start=q_start, k_start=k_start, k_len=k_len, out=o, **kw)
+        assert (o[n:] == 7.0).all()
+        return o[:n] if out is None else out.copy_(o[:n])
+    monkeypatch.setattr(ops, "window_attention", call)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(6, 2, 96), (4, 2, 64), (8, 4, 256), (2, 1, 128), (3, 3, 80), (7, 1, 40), (2, 2, 20), (40, 1, 64)])
+def test_prompt_kernels_on_calls_of_any_size(monkeypatch, nh, nkv, hd, dtype):
+    with_rows_behind(monkeypatch)
+    for window, sinks, cap in ((None, 0, 0.0), (100, 4, 0.0), (33, 0, 20.0), (1, 0, 0.0), (130, 140, 0.0)):
+        test_prompts(nh, nkv, hd, window, sinks, cap, dtype)
+    for lens, prior in (([3, 1, 5, 2], [50, 700, 0, 127]), ([100, 7, 260], [300, 129, 1]), ([64], [999])):
+        test_chunks_behind_a_cache(lens, prior, nh, nkv, hd, 150, 4, 30.0, dtype)
+    test_single_tokens_over_a_cache(nh, nkv, hd, 64, 70, 0.0, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_kernels_on_the_calls_that_can_go_wrong(monkeypatch, dtype):
+    with_rows_behind(monkeypatch)
+    test_queries_without_keys_and_rows_outside_every_sequence(dtype)
+    test_large_scores_and_rising_maxima(dtype)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for where in ("k", "v"):
+            test_non_finite_keys_reach_only_the_rows_that_see_them(dtype, bad, where)
+    for cap in (1e-3, 0.5, 3.0, 1e4, 1e9):
+        test_caps_far_below_and_above_the_scores(dtype, cap)
+    for n in (1, 200):
+        test_strides_and_layouts(dtype, n)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("n", [1, 200])
 def test_strides_and_layouts(dtype, n):
