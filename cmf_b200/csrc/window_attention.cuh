@@ -127,6 +127,7 @@ __device__ __forceinline__ float score(float dot, float scale, float softcap) {
 // tanh(sqrt z) / sqrt z on [0, 0.5625] at Chebyshev points (3e-8, 1.1e-7 with f32 roundings; the quotient below would lose
 // what a large cap makes of a small y); above 1 - 2 / (2^(2 y log2 e) + 1) on the special-function unit.
 constexpr float TANH_POLY_MAX = 0.75f;
+__device__ __forceinline__ float cap_tanh_far(float y) { return 1.0f - __fdividef(2.0f, ex2_approx(y * (2.0f * 1.4426950408889634f)) + 1.0f); }
 __device__ __forceinline__ float cap_tanh(float y) {
     const float z = y * y;
     float q = -0.0047239522f;
@@ -135,8 +136,7 @@ __device__ __forceinline__ float cap_tanh(float y) {
     q = fmaf(q, z, 0.1332551539f);
     q = fmaf(q, z, -0.3333296776f);
     q = fmaf(q, z, 1.0f);
-    const float far = 1.0f - __fdividef(2.0f, ex2_approx(y * (2.0f * 1.4426950408889634f)) + 1.0f);
-    return fabsf(y) <= TANH_POLY_MAX ? y * q : far;
+    return fabsf(y) <= TANH_POLY_MAX ? y * q : cap_tanh_far(y);
 }
 
 // One warp, one (query, head) row, key by key over exactly the keys that the row sees: rows whose tile

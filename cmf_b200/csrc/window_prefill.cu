@@ -102,7 +102,9 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowAttnParams& p, int pos
     return causal & ~passed;
 }
 
-template <typename T, int HDP, int POLY_OF_8, bool CAP>
+// CAP: no soft cap, one of an ordinary size, any (see launch_hdp)
+enum Cap { NO_CAP, CAP_NEAR, CAP_ANY };
+template <typename T, int HDP, int POLY_OF_8, Cap CAP>
 __global__ void __launch_bounds__(THREADS, 1)
 window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowAttnParams p, int tile_tokens, int out_vec) {
@@ -315,6 +317,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         // Soft cap: where all scores of a warp's rows lie in cap_tanh's polynomial range, its coefficients for a score s instead
         // of y = s to_y, times cap log2(e), leave seven packed instructions for the exponents of two scores
         float cap_c[6] = {1.0f, -0.3333296776f, 0.1332551539f, -0.0533498190f, 0.0195937864f, -0.0047239522f};
+        auto tanh_of = [](float y) { return CAP == CAP_NEAR ? cap_tanh_far(y) : cap_tanh(y); };
         if (CAP) {
             float f = cap2 * to_y;
 #pragma unroll
@@ -362,10 +365,10 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
                         mns[(i >> 1) & 3] = fminf(mns[(i >> 1) & 3], fminf(__uint_as_float(v[ch][i]), __uint_as_float(v[ch][i + 1])));
-                small = __all_sync(0xffffffffu, to_y <= 1e3f && fmaxf(mx, -fminf(fminf(mns[0], mns[1]), fminf(mns[2], mns[3]))) * to_y <= TANH_POLY_MAX);
+                small = __all_sync(0xffffffffu, (CAP == CAP_NEAR || to_y <= 1e3f) && fmaxf(mx, -fminf(fminf(mns[0], mns[1]), fminf(mns[2], mns[3]))) * to_y <= TANH_POLY_MAX);
             }
             // the cap keeps the order: the largest capped score is the capped largest score
-            const float m_cand = !CAP ? mx * c : mx == -INFINITY ? mx : cap2 * cap_tanh(mx * to_y);
+            const float m_cand = !CAP ? mx * c : mx == -INFINITY ? mx : cap2 * tanh_of(mx * to_y);
             bad = bad || m_cand != m_cand;
             if (!two && j > 0) {
                 if (!__all_sync(0xffffffffu, mbar_wait(&bars->ref_full[x ^ 1][quarter], (uint32_t)((j - 1) >> 1) & 1u, abort_flag, 9))) { ok = false; break; }
@@ -441,7 +444,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                     const uint32_t bits = r >= used || !masked ? 0xffffffffu : seen_bits(p, pos, j0 + ch * 32);
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        v[ch][i] = bits >> i & 1u ? __float_as_uint(cap_tanh(__uint_as_float(v[ch][i]) * to_y) * cap2) : 0xff800000u;
+                        v[ch][i] = bits >> i & 1u ? __float_as_uint(tanh_of(__uint_as_float(v[ch][i]) * to_y) * cap2) : 0xff800000u;
                 }
                 weights([&](uint64_t sv) { return add_f32x2(sv, nm2); });
             }
@@ -524,7 +527,7 @@ window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     if (threadIdx.x == 0 && bars->abort_flag) atomicCAS(p.status, 0u, 0x900u | bars->abort_flag);
 }
 
-template <typename T, int HDP, int POLY, bool CAP>
+template <typename T, int HDP, int POLY, Cap CAP>
 int launch_form(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, int tile_tokens, cudaStream_t s) {
     static std::atomic<bool> configured[64];
     int dev = 0;
@@ -543,8 +546,12 @@ int launch_form(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensor
 template <typename T, int HDP>
 int launch_hdp(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, int tile_tokens, cudaStream_t s) {
     constexpr int POLY = HDP <= 128 ? 2 : 0;
-    return p.softcap > 0.0f ? launch_form<T, HDP, POLY, true>(tm_q, tm_k, tm_v, p, tile_tokens, s)
-                            : launch_form<T, HDP, POLY, false>(tm_q, tm_k, tm_v, p, tile_tokens, s);
+    // Tiles outside the polynomial's range (masked ones too) take tanh from one quotient, off by up to 2 x 2^-24 of the cap:
+    // 3e-5 at 256, far below a rounding of the weights.  Larger caps, and those so small that powers of scale / cap could
+    // leave the f32 numbers, have a form that goes by the size of each score (8192 tokens, 8 / 4 heads of 256: 348 us, 303).
+    if (!(p.softcap > 0.0f)) return launch_form<T, HDP, POLY, NO_CAP>(tm_q, tm_k, tm_v, p, tile_tokens, s);
+    if (p.softcap <= 256.0f && p.scale <= 1e3f * p.softcap) return launch_form<T, HDP, POLY, CAP_NEAR>(tm_q, tm_k, tm_v, p, tile_tokens, s);
+    return launch_form<T, HDP, POLY, CAP_ANY>(tm_q, tm_k, tm_v, p, tile_tokens, s);
 }
 template <typename T>
 int launch_typed(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, int tile_tokens, cudaStream_t s) {

@@ -401,7 +401,7 @@ def test_many_prompt_tiles_give_the_same_bits(nh, nkv, hd):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("cap", [1e-3, 0.5, 3.0, 1e4, 1e9])
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 3.0, 256.0, 257.0, 1e4, 1e9])
 def test_caps_far_below_and_above_the_scores(dtype, cap):
     """Scores of several units under a cap that they all reach, that some reach, and that none comes near."""
     from cmf_b200 import ops
@@ -414,6 +414,16 @@ def test_caps_far_below_and_above_the_scores(dtype, cap):
             # y P(y^2) or tanhf: 6 roundings of a score of at most 3 x 1.5 x 6 x 6 = 162
             tol = tol + 2 * 6 * 162 * ref.F32 * v.double().abs().max()
         ref.check(out, want, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_of_zero_and_below(dtype):
+    from cmf_b200 import ops
+    for nh, nkv, hd, n in ((4, 2, 64, 200), (2, 1, 256, 1), (24, 24, 32, 200)):
+        q, k, v, _, _, _ = attn_inputs([n], [230 - n], nh, nkv, hd, dtype)
+        for scale, cap in ((0.0, 0.0), (-0.3, 0.0), (-0.2, 2.0), (1e-6, 0.0)):
+            out = ops.window_attention(q, k, v, window=180, sinks=1, scale=scale, softcap=cap)
+            ref.check(out, *ref.window_attention(q, k, v, [n], [0], [230], 180, 1, scale, cap))
 
 
 def with_rows_behind(monkeypatch):
@@ -463,10 +473,11 @@ def test_prompt_kernels_on_the_calls_that_can_go_wrong(monkeypatch, dtype):
     with_rows_behind(monkeypatch)
     test_queries_without_keys_and_rows_outside_every_sequence(dtype)
     test_large_scores_and_rising_maxima(dtype)
+    test_scales_of_zero_and_below(dtype)
     for bad in (float("nan"), float("inf"), -float("inf")):
         for where in ("k", "v"):
             test_non_finite_keys_reach_only_the_rows_that_see_them(dtype, bad, where)
-    for cap in (1e-3, 0.5, 3.0, 1e4, 1e9):
+    for cap in (1e-3, 0.5, 3.0, 256.0, 257.0, 1e4, 1e9):
         test_caps_far_below_and_above_the_scores(dtype, cap)
     for n in (1, 200):
         test_strides_and_layouts(dtype, n)
