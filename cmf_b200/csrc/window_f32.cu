@@ -3,12 +3,14 @@
 //
 // Prompts and chunks: bound by the FMA pipe (4 hd FMA per visible pair).  A block owns 64 rows of one key head.  Scores are 4 x
 // 4 register tiles, outputs 4 x hd / 16, both fed from shared memory: 8 16-byte loads for 64 FMA of a thread.  K and V
-// tiles of 64 keys take turns in two buffers filled by cp.async: V(j) is on its way while S(j) is computed, K(j + 1)
-// while P V(j) is.
+// tiles of 64 keys have a buffer each, filled by cp.async: V(j) is on its way while S(j) is computed, K(j + 1) while P V(j)
+// is.  Only K's rows are padded, so that two blocks of heads up to 128 share an SM (3000 tokens, 16 / 8 heads of 128: 985 us;
+// one block 1130).  Larger tiles of a thread, which read less for each FMA (8 x 8 scores with the dims over four lanes, or 16 x
+// 2 with half of the dims a warp), left too few warps to hide the reads: 1190 and 1092 us.
 // Single tokens: bound by memory, the keys and values once.  A block owns 4 rows of one key head and a share of the key
 // axis (see window_f32_tokens_kernel).
-// Measured: prompts 26 to 33 TFLOP/s (shared-memory loads of the operands share the issue slots with the FMA); 64 sequences x
-// 4096 keys x 4 heads of 256 495 us (4.3 TB/s), one sequence x 256 keys x 8 heads of 128 7.6 us.
+// Measured: prompts 27 to 37 TFLOP/s (half of the FMA pipe's time; the rest is waiting for shared memory); 64 sequences x 4096
+// keys x 4 heads of 256 495 us (4.3 TB/s), one sequence x 256 keys x 8 heads of 128 7.6 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -24,7 +26,7 @@ namespace cg = cooperative_groups;
 constexpr int BM = 64, BN = 64, THREADS = 256, MAX_SPLITS = 8;
 
 template <int HDP>
-constexpr int smem_floats() { return BM * (HDP + 4) + 2 * BN * (HDP + 4) + BM * (BN + 4); }
+constexpr int smem_floats() { return BM * HDP + BN * (HDP + 4) + BN * HDP + BM * BN; }
 
 // 16 bytes, or zeros
 __device__ __forceinline__ void copy16(float* dst, const float* src, bool live) {
@@ -33,13 +35,14 @@ __device__ __forceinline__ void copy16(float* dst, const float* src, bool live) 
 }
 
 template <int HDP>
-__global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_constant__ WindowAttnParams p) {
+__global__ void __launch_bounds__(THREADS, HDP <= 128 ? 2 : 1) window_f32_kernel(const __grid_constant__ WindowAttnParams p) {
     constexpr int A = BM / 16;  // rows of a thread
     extern __shared__ float sm[];
     constexpr int LD = HDP + 4;  // 16-byte rows whose banks shift by four
-    float* Qs = sm;                 // [BM][LD]
-    float* buf = Qs + BM * LD;      // two tiles [BN][LD]: K(j) in the first, V(j) in the second
-    float* Ps = buf + 2 * BN * LD;  // [BM][BN + 4]
+    float* Qs = sm;              // [BM][HDP]
+    float* Ks = Qs + BM * HDP;   // [BN][LD]
+    float* Vs = Ks + BN * LD;    // [BN][HDP]
+    float* Ps = Vs + BN * HDP;   // [BM][BN]
     const int group = p.nh / p.nkv, kvh = blockIdx.x % p.nkv;
     SeqTile st;
     if (!find_tile(p, (gridDim.x - 1 - blockIdx.x) / p.nkv, BM, group, st)) return;
@@ -52,20 +55,20 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
     const KeyTiles kt = key_tiles(p, st, first_i, last_i, BN);
     // rows behind the last key that the block sees are zeros: they may hold anything
     const int end = min(st.k_len, st.k_len - st.q_len + last_i + 1);
-    auto fetch = [&](float* dst, const float* src, int64_t pitch, int j0) {
+    auto fetch = [&](float* dst, int ld, const float* src, int64_t pitch, int j0) {
         for (int t = tid; t < BN * (HDP / 4); t += THREADS) {
             const int j = t / (HDP / 4), d = t % (HDP / 4) * 4;
             const bool live = j0 + j < end && d < p.hd;
-            copy16(dst + j * LD + d, live ? src + (int64_t)(j0 + j) * pitch + d : src, live);
+            copy16(dst + j * ld + d, live ? src + (int64_t)(j0 + j) * pitch + d : src, live);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     for (int t = tid; t < BM * (HDP / 4); t += THREADS) {
         const int r = t / (HDP / 4), d = t % (HDP / 4) * 4, row = r0 + r;
         const bool live = row < rows && d < p.hd;
-        copy16(Qs + r * LD + d, live ? qp + (st.q0 + row / group) * p.q.row + (int64_t)(kvh * group + row % group) * p.q.head + d : qp, live);
+        copy16(Qs + r * HDP + d, live ? qp + (st.q0 + row / group) * p.q.row + (int64_t)(kvh * group + row % group) * p.q.head + d : qp, live);
     }
-    if (kt.count) fetch(buf, kp, p.k.row, kt.at(0) * BN);
+    if (kt.count) fetch(Ks, LD, kp, p.k.row, kt.at(0) * BN);
     float m[A], l[A];
     uint64_t acc[A][HDP / 32];  // pairs of dims
     int pos[A];
@@ -78,10 +81,9 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
 #pragma unroll
         for (int c = 0; c < HDP / 32; ++c) acc[a][c] = 0ull;
     }
-    float *Ks = buf, *Vs = buf + BN * LD;
     for (int it = 0; it < kt.count; ++it) {
         const int j0 = kt.at(it) * BN;
-        fetch(Vs, vp, p.v.row, j0);
+        fetch(Vs, HDP, vp, p.v.row, j0);
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // K(it), and Q
         __syncthreads();
         // even and odd dims in the two halves of a packed sum: one instruction for two FMA
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
         for (int d = 0; d < HDP; d += 4) {
             ulonglong2 qv[A], kv[4];
 #pragma unroll
-            for (int a = 0; a < A; ++a) qv[a] = *reinterpret_cast<const ulonglong2*>(Qs + (ty * A + a) * LD + d);
+            for (int a = 0; a < A; ++a) qv[a] = *reinterpret_cast<const ulonglong2*>(Qs + (ty * A + a) * HDP + d);
 #pragma unroll
             for (int b = 0; b < 4; ++b) kv[b] = *reinterpret_cast<const ulonglong2*>(Ks + (tx + 16 * b) * LD + d);
 #pragma unroll
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
             for (int b = 0; b < 4; ++b) {
                 const float e = expf(s[a][b] - ref);
                 sum += e;
-                Ps[(ty * A + a) * (BN + 4) + tx + 16 * b] = e;
+                Ps[(ty * A + a) * BN + tx + 16 * b] = e;
             }
 #pragma unroll
             for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
         }
         __syncthreads();  // everybody is done with K(it)
         if (it + 1 < kt.count) {
-            fetch(Ks, kp, p.k.row, kt.at(it + 1) * BN);
+            fetch(Ks, LD, kp, p.k.row, kt.at(it + 1) * BN);
             asm volatile("cp.async.wait_group 1;" ::: "memory");
         } else {
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -154,12 +156,12 @@ __global__ void __launch_bounds__(THREADS) window_f32_kernel(const __grid_consta
         for (int j = 0; j < BN; j += 4) {
             float4 pw[A];
 #pragma unroll
-            for (int a = 0; a < A; ++a) pw[a] = *reinterpret_cast<const float4*>(Ps + (ty * A + a) * (BN + 4) + j);
+            for (int a = 0; a < A; ++a) pw[a] = *reinterpret_cast<const float4*>(Ps + (ty * A + a) * BN + j);
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
                 for (int c = 0; c < HDP / 64; ++c) {
-                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(Vs + (j + jj) * LD + c * 64 + tx * 4);
+                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(Vs + (j + jj) * HDP + c * 64 + tx * 4);
 #pragma unroll
                     for (int a = 0; a < A; ++a) {
                         const float w = jj == 0 ? pw[a].x : jj == 1 ? pw[a].y : jj == 2 ? pw[a].z : pw[a].w;
