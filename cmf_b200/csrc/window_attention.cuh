@@ -41,6 +41,15 @@ inline bool window_few_rows(const WindowAttnParams& p, int num_sms) {
     return p.q_rows * (p.nh / p.nkv) <= 16 * (int64_t)p.seqs || window_items(p, 16) <= num_sms;
 }
 
+// Soft caps of the 16-bit forms.  Ordinary ones take tanh from one quotient, off by up to 2 x 2^-24 of the cap: 3e-5 at 256, far
+// below a rounding of the weights (prompts: outside the range of a polynomial whose coefficients hold powers of scale /
+// cap, which must stay f32 numbers).  Others go by the size of each score.  us, ordinary / any: 8192 tokens, 8 / 4 heads of
+// 256 303 / 343; 64 tokens over 4096 keys x 4 heads of 256 160 / 169.
+enum Cap { NO_CAP, CAP_NEAR, CAP_ANY };
+inline Cap cap_form(const WindowAttnParams& p) {
+    return !(p.softcap > 0.0f) ? NO_CAP : p.softcap <= 256.0f && p.scale <= 1e3f * p.softcap ? CAP_NEAR : CAP_ANY;
+}
+
 #ifdef __CUDACC__
 
 struct SeqTile {

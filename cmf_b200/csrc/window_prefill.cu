@@ -102,8 +102,6 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowAttnParams& p, int pos
     return causal & ~passed;
 }
 
-// CAP: no soft cap, one of an ordinary size, any (see launch_hdp)
-enum Cap { NO_CAP, CAP_NEAR, CAP_ANY };
 template <typename T, int HDP, int POLY_OF_8, Cap CAP>
 __global__ void __launch_bounds__(THREADS, 1)
 window_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -546,12 +544,11 @@ int launch_form(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensor
 template <typename T, int HDP>
 int launch_hdp(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, int tile_tokens, cudaStream_t s) {
     constexpr int POLY = HDP <= 128 ? 2 : 0;
-    // Tiles outside the polynomial's range (masked ones too) take tanh from one quotient, off by up to 2 x 2^-24 of the cap:
-    // 3e-5 at 256, far below a rounding of the weights.  Larger caps, and those so small that powers of scale / cap could
-    // leave the f32 numbers, have a form that goes by the size of each score (8192 tokens, 8 / 4 heads of 256: 348 us, 303).
-    if (!(p.softcap > 0.0f)) return launch_form<T, HDP, POLY, NO_CAP>(tm_q, tm_k, tm_v, p, tile_tokens, s);
-    if (p.softcap <= 256.0f && p.scale <= 1e3f * p.softcap) return launch_form<T, HDP, POLY, CAP_NEAR>(tm_q, tm_k, tm_v, p, tile_tokens, s);
-    return launch_form<T, HDP, POLY, CAP_ANY>(tm_q, tm_k, tm_v, p, tile_tokens, s);
+    switch (cap_form(p)) {
+        case NO_CAP: return launch_form<T, HDP, POLY, NO_CAP>(tm_q, tm_k, tm_v, p, tile_tokens, s);
+        case CAP_NEAR: return launch_form<T, HDP, POLY, CAP_NEAR>(tm_q, tm_k, tm_v, p, tile_tokens, s);
+        default: return launch_form<T, HDP, POLY, CAP_ANY>(tm_q, tm_k, tm_v, p, tile_tokens, s);
+    }
 }
 template <typename T>
 int launch_typed(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, int tile_tokens, cudaStream_t s) {

@@ -83,7 +83,7 @@ __device__ __forceinline__ uint32_t tile_at(uint32_t base, int row, int unit) {
     return base + (unit >> 3) * (KEYS * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
 }
 
-template <typename T, int HDP, bool CAP, int W>
+template <typename T, int HDP, Cap CAP, int W>
 __global__ void __launch_bounds__(32 * (1 + W), (Smem<HDP, W>::PER_SM))
 window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowAttnParams p, int splits) {
     using L = Smem<HDP, W>;
@@ -208,7 +208,7 @@ window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    x[n][e] = CAP ? cap2 * cap_tanh(cur[n][e] * to_y) : cur[n][e] * sc;
+                    x[n][e] = CAP ? cap2 * (CAP == CAP_NEAR ? cap_tanh_far(cur[n][e] * to_y) : cap_tanh(cur[n][e] * to_y)) : cur[n][e] * sc;
             if (j0 + 15 > pos_min || ((int64_t)seen_last - j0 >= p.window && j0 + 16 > p.sinks)) {  // some row does not see all 16 keys
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
@@ -367,7 +367,7 @@ window_tokens_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     if (splits > 1) cluster.sync();  // nobody's shared memory goes away while another block reads it
 }
 
-template <typename T, int HDP, bool CAP, int W>
+template <typename T, int HDP, Cap CAP, int W>
 int launch_form(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, cudaStream_t s) {
     static std::atomic<int> clusters_of[64][MAX_SPLITS + 1];  // clusters that run at once, a property of the device
     int dev = 0;
@@ -403,6 +403,14 @@ int launch_form(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAt
     CMFC_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm_k, tm_v, p, splits));
     return OK;
 }
+template <typename T, int HDP, int W>
+int launch_warps(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, cudaStream_t s) {
+    switch (cap_form(p)) {
+        case NO_CAP: return launch_form<T, HDP, NO_CAP, W>(tm_k, tm_v, p, s);
+        case CAP_NEAR: return launch_form<T, HDP, CAP_NEAR, W>(tm_k, tm_v, p, s);
+        default: return launch_form<T, HDP, CAP_ANY, W>(tm_k, tm_v, p, s);
+    }
+}
 template <typename T, int HDP>
 int launch_hdp(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, int num_sms, cudaStream_t s) {
     // A warp's step over 16 keys is a chain of about 1200 clocks whatever else runs.  Few items: eight warps a block, one
@@ -411,9 +419,9 @@ int launch_hdp(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAtt
     // with eight warps 188).  Heads of 256 leave room for the tiles of four warps.
     if constexpr (HDP <= 128) {
         if (window_items(p, ROWS) <= num_sms / 2)
-            return p.softcap > 0.0f ? launch_form<T, HDP, true, 8>(tm_k, tm_v, p, s) : launch_form<T, HDP, false, 8>(tm_k, tm_v, p, s);
+            return launch_warps<T, HDP, 8>(tm_k, tm_v, p, s);
     }
-    return p.softcap > 0.0f ? launch_form<T, HDP, true, 4>(tm_k, tm_v, p, s) : launch_form<T, HDP, false, 4>(tm_k, tm_v, p, s);
+    return launch_warps<T, HDP, 4>(tm_k, tm_v, p, s);
 }
 template <typename T>
 int launch_typed(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowAttnParams& p, int num_sms, cudaStream_t s) {
