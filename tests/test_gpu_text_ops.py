@@ -635,6 +635,54 @@ def test_calls_on_other_streams_in_two_graphs_and_at_once():
             assert torch.equal(x1, x2)
 
 
+def test_threads_call_at_once_each_on_its_stream():
+    import threading
+    from cmf_b200 import ops
+    g = gen(11)
+    q, k, v, _, _, where = attn_inputs([1, 3, 90], [300, 20, 500], 6, 2, 96, torch.bfloat16)
+    x = randn(g, 40, 512, dtype=torch.float16)
+    w, s = torch.randint(-127, 128, (256, 512), generator=g, device="cuda", dtype=torch.int8), torch.rand(256, generator=g, device="cuda")
+    qkv, nq, nk, cos, sin, pos = rope_inputs(65, 6, 2, 64, 64, torch.float32)
+
+    def every():
+        return [ops.window_attention(q, k, v, window=100, **where), ops.i8_linear(x, w, s), *ops.quantize_rows(x),
+                *ops.qk_norm_rope(qkv[:, :6], qkv[:, 6:8], nq, nk, cos, sin, positions=pos)]
+    want = every()
+    torch.cuda.synchronize()
+    got, errors = [], []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got.append(every())
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # reported by the test's own thread
+            errors.append(e)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and len(got) == 80
+    assert all(torch.equal(a, b) for outs in got for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sequences_that_share_key_rows(dtype):
+    """A common beginning of several sequences, read by all of them in place."""
+    from cmf_b200 import ops
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    g = gen(12)
+    for lens in ([1, 1, 1, 1], [5, 40, 1, 70]):
+        q = randn(g, sum(lens), 4, 64, dtype=dtype)
+        k, v = randn(g, 300, 2, 64, dtype=dtype), randn(g, 300, 2, 64, dtype=dtype)
+        starts, total = [0, 0, 10, 0], [300, 250, 100, 300]
+        qs = [sum(lens[:i]) for i in range(5)]
+        out = ops.window_attention(q, k, v, window=200, sinks=7, q_start=i32(*qs), k_start=i32(*starts), k_len=i32(*total))
+        ref.check(out, *ref.window_attention(q, k, v, lens, starts, total, 200, 7, 0.125, 0.0))
+
+
 CAPTURE = """
 import torch
 from cmf_b200 import ops
