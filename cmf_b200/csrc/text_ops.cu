@@ -54,13 +54,15 @@ bool distinct(int64_t rows, int64_t heads, int64_t hd, int64_t row, int64_t head
     if (rows > 1 && heads > 1) {
         const bool heads_inside = head <= row;
         const int64_t lo = heads_inside ? head : row, lo_n = heads_inside ? heads : rows, hi = heads_inside ? row : head;
-        return lo >= hd && hi >= (lo_n - 1) * lo + hd;
+        return lo >= hd && (hi - hd) / lo >= lo_n - 1;
     }
     if (rows > 1) return row >= hd;
     return heads <= 1 || head >= hd;
 }
-constexpr int64_t MAX_STRIDE = (int64_t)1 << 40;  // rows x stride stays far below 2^63
+constexpr int64_t MAX_STRIDE = (int64_t)1 << 40;  // in a tensor that exists, rows x stride stays far below 2^63
 bool stride_ok(int64_t s) { return s >= 0 && s < MAX_STRIDE; }
+
+bool on_elements(const void* p, int elem) { return reinterpret_cast<uintptr_t>(p) % (size_t)elem_bytes(elem) == 0; }
 
 template <class F>
 int guarded(F f) {
@@ -77,6 +79,7 @@ int quantize_rows_impl(int device, const void* x, int elem, size_t rows, size_t 
     NEED(rows <= MOST && cols >= 1 && cols <= MOST, "quantize_rows: rows must be at most 2^31 - 1024, cols in [1, 2^31 - 1024]");
     if (rows == 0) return OK;
     NEED(x && q && scale, "quantize_rows: null pointer");
+    NEED(on_elements(x, elem) && on_elements(scale, ET_F32), "quantize_rows: a pointer is off its element's boundary");
     NEED(stride_ok(ldx) && stride_ok(ldq) && (rows == 1 || (ldx >= (int64_t)cols && ldq >= (int64_t)cols)),
          "quantize_rows: a row pitch is shorter than a row");
     OnDevice on;
@@ -112,6 +115,7 @@ int i8_matmat_impl(int device, const int8_t* xq, int64_t ldx, const float* xs, c
     if (cols > (size_t)I8_MAX_K) return fail(ERR_UNSUPPORTED, "i8_matmat: cols above 131071 could overflow the 32-bit sum");
     if (b == 0) return OK;
     NEED(xq && xs && wq && ws && y, "i8_matmat: null pointer");
+    NEED(on_elements(xs, ET_F32) && on_elements(ws, ET_F32) && on_elements(y, elem), "i8_matmat: a pointer is off its element's boundary");
     NEED(stride_ok(ldx) && stride_ok(ldw) && stride_ok(ldy), "i8_matmat: bad row pitch");
     NEED((b == 1 || ldx >= (int64_t)cols) && (rows == 1 || ldw >= (int64_t)cols) && (b == 1 || ldy >= (int64_t)rows),
          "i8_matmat: a row pitch is shorter than a row");
@@ -141,6 +145,7 @@ int i8_linear_impl(int device, const void* x, int elem, int64_t ldx, const int8_
     if (cols > (size_t)I8_MAX_K) return fail(ERR_UNSUPPORTED, "i8_linear: cols above 131071 could overflow the 32-bit sum");
     if (b == 0) return OK;
     NEED(x && wq && ws && y, "i8_linear: null pointer");
+    NEED(on_elements(x, elem) && on_elements(ws, ET_F32) && on_elements(y, y_elem), "i8_linear: a pointer is off its element's boundary");
     NEED(stride_ok(ldx) && stride_ok(ldw) && stride_ok(ldy), "i8_linear: bad row pitch");
     NEED((b == 1 || ldx >= (int64_t)cols) && (rows == 1 || ldw >= (int64_t)cols) && (b == 1 || ldy >= (int64_t)rows),
          "i8_linear: a row pitch is shorter than a row");
@@ -182,6 +187,10 @@ int qk_norm_rope_impl(int device, const cmfc_qk_norm_rope_args* a, cudaStream_t 
     NEED((!a->nh || (a->q && a->q_out && a->norm_q)) && (!a->nkv || (a->k && a->k_out && a->norm_k)) &&
              (!a->rot || (a->cos_t && a->sin_t)),
          "qk_norm_rope: null pointer");
+    NEED(on_elements(a->q, a->elem) && on_elements(a->k, a->elem) && on_elements(a->q_out, a->elem) && on_elements(a->k_out, a->elem) &&
+             on_elements(a->norm_q, ET_F32) && on_elements(a->norm_k, ET_F32) && on_elements(a->cos_t, ET_F32) && on_elements(a->sin_t, ET_F32) &&
+             reinterpret_cast<uintptr_t>(a->positions) % (a->positions_64 ? 8 : 4) == 0,
+         "qk_norm_rope: a pointer is off its element's boundary");
     const int64_t st[8] = {a->q_row, a->q_head, a->k_row, a->k_head, a->q_out_row, a->q_out_head, a->k_out_row, a->k_out_head};
     for (int64_t v : st) NEED(stride_ok(v), "qk_norm_rope: bad stride");
     NEED(distinct((int64_t)a->n, a->nh, a->hd, a->q_out_row, a->q_out_head) && distinct((int64_t)a->n, a->nkv, a->hd, a->k_out_row, a->k_out_head),
@@ -224,6 +233,9 @@ int window_attention_impl(int device, const cmfc_window_attention_args* a, cudaS
     NEED(packed ? a->seqs <= 1u << 30 : a->seqs == 1, "window_attention: without q_start there is one sequence");
     if (a->q_rows == 0 || a->seqs == 0) return OK;
     NEED(a->q && a->out && (a->k_rows == 0 || (a->k && a->v)), "window_attention: null pointer");
+    NEED(on_elements(a->q, a->elem) && on_elements(a->k, a->elem) && on_elements(a->v, a->elem) && on_elements(a->out, a->elem) &&
+             on_elements(a->q_start, ET_F32) && on_elements(a->k_start, ET_F32) && on_elements(a->k_len, ET_F32),
+         "window_attention: a pointer is off its element's boundary");
     const int64_t st[8] = {a->q_row, a->q_head, a->k_row, a->k_head, a->v_row, a->v_head, a->out_row, a->out_head};
     for (int64_t v : st) NEED(stride_ok(v), "window_attention: bad stride");
     NEED(distinct((int64_t)a->q_rows, a->nh, a->hd, a->out_row, a->out_head), "window_attention: heads of the output overlap");

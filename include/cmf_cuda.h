@@ -274,7 +274,8 @@ int cmfc_matmat_device_noalloc(cmfc_model* m, int64_t idx, const float* d_x, siz
  * same kind above: 8-bit products beside q8_matmat, windowed attention beside dit_attention, head norms
  * with the rotation beside the pass that the denoiser runs inside its blocks.
  *
- * All pointers are memory of `device`; strides and pitches are in elements.  The work is enqueued on
+ * All pointers are memory of `device` on their element's boundary; strides and pitches are in elements; outputs
+ * overlap no input unless an entry says so.  The work is enqueued on
  * `stream` (a cudaStream_t, NULL: the legacy default stream) and the call returns at once: inputs and
  * outputs belong to the call until that stream has passed it.  A call may be captured into a CUDA graph once
  * the device has a context (any earlier call on it, or cmfc_set_device).  Nothing is kept between
@@ -288,8 +289,9 @@ int cmfc_matmat_device_noalloc(cmfc_model* m, int64_t idx, const float* d_x, siz
 #define CMFC_ET_BF16 2
 
 /* Rows to 8 bits: scale[r] = max_c |x[r, c]| * (1 / 127), q[r, c] = rint(x[r, c] / scale[r]) (ties to even;
- * the constant, the product and the quotient each rounded to f32).  A row of zeros gives scale 0 and levels 0; a row that holds an infinity or a NaN gives
- * scale NaN and levels 0.  x [rows, cols] of type `elem`, pitch ldx; q pitch ldq; scale [rows]. */
+ * the constant, the product and the quotient each rounded to f32).  A row of zeros gives scale 0 and levels 0; a
+ * row that holds an infinity or a NaN gives scale NaN and levels 0.  x [rows, cols] of type `elem`, pitch ldx; q pitch
+ * ldq; scale [rows]. */
 int cmfc_quantize_rows(int device, const void* x, int elem, size_t rows, size_t cols, int64_t ldx, int8_t* q, int64_t ldq,
                        float* scale, void* stream);
 /* y[m, n] = (sum_k xq[m, k] wq[n, k]) * (x_scale[m] * w_scale[n]): xq [b, cols], wq [rows, cols] (a q8_row

@@ -107,7 +107,8 @@ def test_library_refuses_before_any_device_call():
     for kw, code in [(dict(elem=3), -1), (dict(nh=0, nkv=0), -1), (dict(hd=0, rot=0), -1), (dict(rot=15), -1), (dict(rot=18), -1),
                      (dict(eps=-1.0), -1), (dict(eps=float("nan")), -1), (dict(ptrs=[0] * 9), -1), (dict(table=0), -1),
                      (dict(strides=[32, 16, 32, 16, 32, 8, 32, 16]), -1), (dict(strides=[-32, 16] + [32, 16] * 3), -1),
-                     (dict(n=2 ** 30), -2)]:
+                     (dict(ptrs=[258] + [256] * 8), -1), (dict(ptrs=[256] * 8 + [260], pos64=1), -1), (dict(ptrs=[256] * 7 + [254, 256], elem=2), -1),
+                     (dict(strides=[32, 16] * 2 + [2 ** 39, 16, 2 ** 39, 2 ** 39 + 8], n=2 ** 28), -1), (dict(n=2 ** 30), -2)]:
         assert L.cmfc_qk_norm_rope(0, rope_args(**kw), None) == code, (kw, L.cmfc_last_error())
     assert L.cmfc_qk_norm_rope(0, None, None) == -1
     assert L.cmfc_qk_norm_rope(0, rope_args(n=0), None) == 0
@@ -122,18 +123,21 @@ def test_library_refuses_before_any_device_call():
     for kw, code in [(dict(elem=-1), -1), (dict(nh=3), -1), (dict(nkv=0), -1), (dict(hd=0), -1), (dict(hd=257), -2), (dict(scale=float("inf")), -1),
                      (dict(softcap=-1.0), -1), (dict(seqs=2), -1), (dict(ptrs=[256] * 4 + [256, 0, 0]), -1), (dict(ptrs=[0] * 7), -1),
                      (dict(q_rows=2 ** 31), -1), (dict(k_rows=2 ** 31 - 100), -1), (dict(q_rows=2 ** 30), -1), (dict(strides=[64, 16, 32, 16, 32, 16, 64, 8]), -1),
-                     (dict(strides=[64, 16, 32, -16, 32, 16, 64, 16]), -1)]:
+                     (dict(strides=[64, 16, 32, -16, 32, 16, 64, 16]), -1), (dict(ptrs=[256, 258, 256, 256, 0, 0, 0]), -1),
+                     (dict(ptrs=[256, 257, 256, 256, 0, 0, 0], elem=1), -1), (dict(ptrs=[256] * 4 + [256, 258, 256]), -1)]:
         assert L.cmfc_window_attention(0, attn_args(**kw), None) == code, (kw, L.cmfc_last_error())
     assert L.cmfc_window_attention(0, None, None) == -1
     assert L.cmfc_window_attention(0, attn_args(q_rows=0), None) == 0
 
     q = lambda **kw: L.cmfc_quantize_rows(*{**dict(dev=0, x=p, elem=0, rows=4, cols=8, ldx=8, q=p, ldq=8, s=p, st=None), **kw}.values())  # noqa: E731
     assert q(elem=9) == -1 and q(cols=0) == -1 and q(x=None) == -1 and q(ldx=7) == -1 and q(ldq=7) == -1 and q(ldx=-8) == -1
+    assert q(x=C.c_void_p(258)) == -1 and q(s=C.c_void_p(257)) == -1
     assert q(rows=0) == 0 and q(rows=2 ** 31 - 1) == -1 and q(cols=2 ** 31, ldx=2 ** 31, ldq=2 ** 31) == -1
     m = lambda **kw: L.cmfc_i8_matmat(*{**dict(dev=0, x=p, ldx=8, xs=p, w=p, ldw=8, ws=p, b=4, rows=4, cols=8, y=p, elem=0, ldy=4, st=None),  # noqa: E731
                                         **kw}.values())
     assert m(elem=9) == -1 and m(rows=0) == -1 and m(cols=0) == -1 and m(w=None) == -1 and m(ldx=7) == -1 and m(ldy=3) == -1
     assert m(cols=131072, ldx=131072, ldw=131072) == -2
+    assert m(ws=C.c_void_p(258)) == -1 and m(y=C.c_void_p(258)) == -1 and m(y=C.c_void_p(257), elem=2) == -1
     assert m(b=0) == 0
     # the workspace of i8_linear: none for a few short aligned tokens, levels and scales otherwise
     assert L.cmfc_i8_linear_workspace(p, 2, 64, p, 64, 1, 8, 64) == 0
