@@ -11,13 +11,14 @@
 // 16-byte chunks of a head that hold both members of its pairs (neighbouring chunks, or the same
 // chunk of either half), so the rotation needs no exchange between lanes; a head takes a group of
 // 4 to 32 lanes and a warp works on 32 / group items.  Measured, 8704 tokens x 32 heads of 96: f32 37 to 40 us (5.6 TB/s, 0.85 of
-// a copy's rate); bf16 27 us (4.1 TB/s), where the conversions and the reduction of 32 values a lane hold up the loads; one
+// a copy's rate); bf16 27 us (4.1 TB/s), where the conversions and the reduction of 16 values a lane and head hold up the loads; one
 // token 2.2 us.  Items by a 2-D grid, a loop over tokens and a register cap were each slower.
 #include "i8_gemm.cuh"
 
 namespace cmfc {
 namespace {
 
+// heads in flight of a lane; 2 / 3 / 8 instead: 17.7 / 18.3 / 24.4 us against 16.5 (5531 tokens, 8 + 4 heads of 256, f16)
 constexpr int HEADS_PER_ITEM = 4;
 
 // N (a multiple of 4) values from a 16-byte aligned place

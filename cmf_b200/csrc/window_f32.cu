@@ -9,7 +9,7 @@
 // 2 with half of the dims a warp), left too few warps to hide the reads: 1190 and 1092 us.
 // Single tokens: bound by memory, the keys and values once.  A block owns 4 rows of one key head and a share of the key
 // axis (see window_f32_tokens_kernel).
-// Measured: prompts 27 to 37 TFLOP/s (half of the FMA pipe's time; the rest is waiting for shared memory); 64 sequences x 4096
+// Measured: prompts 27 to 37 TFLOP/s (FMA pipe half to two thirds busy; the rest is waiting for shared memory); 64 sequences x 4096
 // keys x 4 heads of 256 495 us (4.3 TB/s), one sequence x 256 keys x 8 heads of 128 7.6 us.
 #include <cooperative_groups.h>
 
